@@ -24,6 +24,22 @@ int a4c_launch_gemm_float(const void* A, long long a_rs, long long a_cs, long lo
 int a4c_launch_add_float(const void* a, long long lda, const void* b, long long ldb, void* out, long long ldo,
                          long long rows, long long cols, int kind, cudaStream_t stream);
 
+// MXFP4 (mx_quant.cu, dense_mx.cu): codes with pitches in elements (multiples of 32), scale tiles of 512 bytes.
+int a4c_launch_quantize_mx(const void* x, int kind, long long ldx, uint8_t* codes, long long ldc, uint8_t* scales,
+                           long long rows, long long cols, cudaStream_t stream);
+int a4c_launch_dequantize_mx(const uint8_t* codes, long long ldc, const uint8_t* scales, void* y, int kind, long long ldy,
+                             long long rows, long long cols, cudaStream_t stream);
+struct A4cMxDense {
+    const uint8_t* a; long long lda; const uint8_t* sa;
+    const uint8_t* w; long long ldw; const uint8_t* sw;      // Dense weights, or the gate's
+    const uint8_t* wu; long long ldu; const uint8_t* su;     // the other projection's, or null for a plain Dense
+    const float* bias; const float* bias_u;
+    void* y; int out_kind; long long ldy; uint8_t* ys;
+    long long M; int K, N;
+    int act;                                                 // a plain Dense knows none (0) and ReLU (1)
+};
+int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stream);
+
 // tcgen05 / TMA / TMEM int8 GEMM: A [M,K] K-contiguous, Wt [N,K] K-contiguous.
 // cta_pair = 0: one CTA per 128x256 tile; 1: a CTA pair (cta_group::2) per 256x256 tile.
 int a4c_launch_dense_tc(const void* A, long long lda, const void* Wt, long long ldw, const int32_t* bias,

@@ -263,6 +263,88 @@ int a4c_add_f(const void* a, int64_t lda, const void* b, int64_t ldb, void* out,
     return finish();
 }
 
+int64_t a4c_mx_scale_bytes(int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    return ((rows - 1) / 128 + 1) * ((cols - 1) / 128 + 1) * 512;
+}
+
+// codes and scales of one MXFP4 operand
+static int check_mx(const uint8_t* codes, int64_t ld, const uint8_t* scales, int64_t cols) {
+    if (codes == nullptr || scales == nullptr || ld < cols) return A4C_ERR_INVALID_ARG;
+    if ((((uintptr_t)codes | (uintptr_t)scales) & 15u) || ld % 32) return A4C_ERR_ALIGNMENT;
+    return A4C_OK;
+}
+// a bfloat16 (0) or float32 (1) tensor
+static int check_f(const void* x, int fdtype, int64_t ld, int64_t cols) {
+    if (x == nullptr || ld < cols || (fdtype != 0 && fdtype != 1)) return A4C_ERR_INVALID_ARG;
+    return ((uintptr_t)x & (fdtype == 0 ? 1u : 3u)) ? A4C_ERR_ALIGNMENT : A4C_OK;
+}
+
+int a4c_quantize_mx(const void* x, int fdtype, int64_t ldx, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t rows,
+                    int64_t cols, void* stream) {
+    if (rows < 0 || cols <= 0) return A4C_ERR_INVALID_ARG;
+    int rc = check_f(x, fdtype, ldx, cols);
+    if (rc == A4C_OK) rc = check_mx(codes, ldc, scales, cols);
+    if (rc != A4C_OK) return rc;
+    if (rows == 0) return A4C_OK;
+    rc = a4c_launch_quantize_mx(x, fdtype, ldx, codes, ldc, scales, rows, cols, (cudaStream_t)stream);
+    if (rc != A4C_OK) { if (rc == A4C_ERR_CUDA) note(cudaGetLastError()); return rc; }
+    return finish();
+}
+
+int a4c_dequantize_mx(const uint8_t* codes, int64_t ldc, const uint8_t* scales, void* y, int fdtype, int64_t ldy, int64_t rows,
+                      int64_t cols, void* stream) {
+    if (rows < 0 || cols <= 0) return A4C_ERR_INVALID_ARG;
+    int rc = check_f(y, fdtype, ldy, cols);
+    if (rc == A4C_OK) rc = check_mx(codes, ldc, scales, cols);
+    if (rc != A4C_OK) return rc;
+    if (rows == 0) return A4C_OK;
+    rc = a4c_launch_dequantize_mx(codes, ldc, scales, y, fdtype, ldy, rows, cols, (cudaStream_t)stream);
+    if (rc != A4C_OK) { if (rc == A4C_ERR_CUDA) note(cudaGetLastError()); return rc; }
+    return finish();
+}
+
+static int dense_mx_any(const A4cMxDense& d, void* stream) {
+    if (d.M < 0 || d.K <= 0 || d.N <= 0 || d.M > 2147483647LL - 256 || d.N > 2147483647 - 256 || d.K > 2147483647 - 256) return A4C_ERR_INVALID_ARG;
+    int rc = check_mx(d.a, d.lda, d.sa, d.K);
+    if (rc == A4C_OK) rc = check_mx(d.w, d.ldw, d.sw, d.K);
+    if (rc == A4C_OK && d.wu != nullptr) rc = check_mx(d.wu, d.ldu, d.su, d.K);
+    if (rc == A4C_OK) {
+        if (d.out_kind == 3) rc = check_mx((const uint8_t*)d.y, d.ldy, d.ys, d.N);
+        else rc = d.ys != nullptr ? A4C_ERR_INVALID_ARG : check_f(d.y, d.out_kind, d.ldy, d.N);
+    }
+    if (rc == A4C_OK && (((uintptr_t)d.bias | (uintptr_t)d.bias_u) & 3u)) rc = A4C_ERR_ALIGNMENT;
+    if (rc != A4C_OK) return rc;
+    if (d.M == 0) return A4C_OK;
+    int* word = status_word();
+    if (word == nullptr) return A4C_ERR_CUDA;
+    rc = a4c_launch_dense_mx(d, word, (cudaStream_t)stream);
+    if (rc != A4C_OK) { if (rc == A4C_ERR_CUDA) note(cudaGetLastError()); return rc; }
+    return finish();
+}
+
+int a4c_dense_mx(const uint8_t* A, int64_t lda, const uint8_t* A_scales, const uint8_t* Wt, int64_t ldw, const uint8_t* W_scales,
+                 const float* bias, void* Y, int fdtype, int64_t ldy, uint8_t* Y_scales, int64_t M, int K, int N, int relu,
+                 void* stream) {
+    A4cMxDense d;
+    d.a = A; d.lda = lda; d.sa = A_scales; d.w = Wt; d.ldw = ldw; d.sw = W_scales; d.wu = nullptr; d.ldu = 0; d.su = nullptr;
+    d.bias = bias; d.bias_u = nullptr; d.y = Y; d.out_kind = fdtype; d.ldy = ldy; d.ys = Y_scales; d.M = M; d.K = K; d.N = N;
+    d.act = relu ? A4C_ACT_RELU : A4C_ACT_NONE;
+    return dense_mx_any(d, stream);
+}
+
+int a4c_gated_dense_mx(const uint8_t* A, int64_t lda, const uint8_t* A_scales, const uint8_t* Wg, int64_t ldg,
+                       const uint8_t* Wg_scales, const uint8_t* Wu, int64_t ldu, const uint8_t* Wu_scales, const float* bias_g,
+                       const float* bias_u, void* Y, int fdtype, int64_t ldy, uint8_t* Y_scales, int64_t M, int K, int N,
+                       int activation, void* stream) {
+    if (Wu == nullptr || activation < A4C_ACT_NONE || activation > A4C_ACT_SIGMOID) return A4C_ERR_INVALID_ARG;
+    A4cMxDense d;
+    d.a = A; d.lda = lda; d.sa = A_scales; d.w = Wg; d.ldw = ldg; d.sw = Wg_scales; d.wu = Wu; d.ldu = ldu; d.su = Wu_scales;
+    d.bias = bias_g; d.bias_u = bias_u; d.y = Y; d.out_kind = fdtype; d.ldy = ldy; d.ys = Y_scales; d.M = M; d.K = K; d.N = N;
+    d.act = activation;
+    return dense_mx_any(d, stream);
+}
+
 int a4c_attention_heads_i8_supported(const int8_t* q, int64_t ldq, int64_t stride_q, int64_t hstride_q, const int8_t* k,
                                      int64_t ldk, int64_t stride_k, int64_t hstride_k, const int8_t* v, int64_t ldv,
                                      int64_t stride_v, int64_t hstride_v, const int8_t* out, int64_t ldo, int64_t stride_o,

@@ -1,0 +1,398 @@
+// Dense and gated Dense over MXFP4 operands for any number of rows: the tile kernel.
+//
+//   Dense:  Y[m,n] = relu?(sum_k A[m,k] W[n,k] + bias[n])
+//   gated:  Y[m,n] = act(sum_k A[m,k] Wg[n,k] + bg[n]) * (sum_k A[m,k] Wu[n,k] + bu[n])
+//
+// Products of block-scaled E2M1 values on tcgen05.mma kind::mxf4 (the scales are applied inside the instruction),
+// float32 accumulators in TMEM, bias, activation and the rounding to the output type (bfloat16, float32, or MXFP4 with
+// its scales) in the epilogue.
+//
+// With few rows the time is the weights' way out of memory, so the weights are the M operand here (128 of them to a
+// tile) and the rows of A the N operand (16 to 128): a tile fetches 16 KB of weights for 2 KB of A at 16 rows, where the
+// other way round every tile would carry 128 mostly empty rows.  When there are fewer tiles than SMs the reduction is
+// split over a cluster of up to 8 CTAs: each leaves its partial tile in its own shared memory and the ranks add them up
+// in rank order over distributed shared memory, so the result does not depend on timing and no workspace exists.
+//
+// One tile per CTA: warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue.  A stage is 256 values of K: 128-byte
+// swizzled rows of codes and the scale tiles, which tcgen05.cp moves on to TMEM ahead of the stage's MMAs (the tensor
+// pipe takes both in issue order).  Every wait is bounded.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "a4c_common.cuh"
+#include "a4c_kernels.h"
+#include "mx_common.cuh"
+
+namespace {
+
+using namespace tc;
+
+constexpr int BN = 128;                       // output features per tile
+constexpr int MAX_T = 128;                    // rows of A per tile, at most
+constexpr int BK = 256;                       // K values per stage (128 bytes of codes)
+constexpr int W_BYTES = BN * BK / 2;
+constexpr int SF_BYTES = 2 * mx::TILE_BYTES;  // scales of 128 rows x 256 values
+constexpr int NUM_THREADS = 192;
+constexpr int MAX_STAGES = 12;
+constexpr int MAX_SPLIT = 8;                  // portable cluster size
+constexpr int SMEM_BUDGET = 200 * 1024;
+constexpr size_t ONE_PER_SM = 116 * 1024;
+
+struct Tail {
+    uint64_t full[MAX_STAGES];
+    uint64_t empty[MAX_STAGES];
+    uint64_t done;
+    uint32_t tmem_base;
+    volatile int abort_flag;
+};
+
+struct Args {
+    const uint8_t* sa;               // scale tiles
+    const uint8_t* sw[2];
+    const float* bias[2];
+    void* Y; long long ldy;          // elements
+    uint8_t* ys; long long y_across; // MXFP4 output: scale tiles
+    long long M;
+    int N, K;
+    int k_tiles;                     // scale tiles across K
+    int num_kb;                      // stages of the whole reduction
+    int t;                           // rows of A per tile (multiple of 16)
+    int split;                       // CTAs per tile (cluster size)
+    int num_n_tiles;
+    int stages, stage_bytes;
+    int out_kind, act;
+    uint32_t idesc;
+    int* status;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// One value of row m and feature n (this lane's), complete over K; the 32 lanes of a warp hold 32 neighbouring
+// features, which for an MXFP4 output are one block.  Called by whole warps with the same m.
+__device__ __forceinline__ void store_value(const Args& g, long long m, int n, float v) {
+    if (g.out_kind == mx::KIND_BF16) {
+        if (n < g.N) reinterpret_cast<__nv_bfloat16*>(g.Y)[m * g.ldy + n] = __float2bfloat16_rn(v);
+    } else if (g.out_kind == mx::KIND_F32) {
+        if (n < g.N) reinterpret_cast<float*>(g.Y)[m * g.ldy + n] = v;
+    } else {
+        const int lane = threadIdx.x & 31;
+        const int n0 = n - lane;
+        if (n >= g.N) v = 0.0f;
+        const uint32_t s = mx::scale_code(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu));
+        const float q[8] = {v * mx::inverse_scale(s == 255u ? 0u : s), 0, 0, 0, 0, 0, 0, 0};
+        uint32_t w = s == 255u ? 0u : (mx::pack_e2m1(q) & 15u) << (4 * (lane & 7));
+        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 1);
+        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 2);
+        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+        if (n0 < g.N) {
+            uint8_t* dst = reinterpret_cast<uint8_t*>(g.Y) + (m * g.ldy + n0) / 2;
+            const int bytes = (min(32, g.N - n0) + 1) >> 1;
+            // lane 8 j holds the word of features 8 j .. 8 j + 7
+            if ((lane & 7) == 0) {
+                const int b0 = lane >> 1;
+                if (b0 + 4 <= bytes) *reinterpret_cast<uint32_t*>(dst + b0) = w;
+                else for (int b = b0; b < bytes; ++b) dst[b] = (uint8_t)(w >> (8 * (b - b0)));
+            }
+            if (lane == 0) g.ys[mx::scale_offset(m, n0 >> 5, g.y_across)] = (uint8_t)s;
+        } else if ((n0 >> 5) < (int)g.y_across * mx::TILE_BLOCKS && lane == 0) {
+            g.ys[mx::scale_offset(m, n0 >> 5, g.y_across)] = 0;   // places beyond the tensor
+        }
+    }
+}
+
+template <bool GATED>
+__device__ __forceinline__ float finish_value(const Args& g, float a, float u, float ba, float bu) {
+    a += ba;
+    if (GATED) return mx::activate(a, g.act) * (u + bu);
+    return g.act == mx::ACT_RELU && a < 0.0f ? 0.0f : a;
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                const __grid_constant__ CUtensorMap map_u, Args g) {
+    constexpr int NW = GATED ? 2 : 1;
+    constexpr int SF_COLS = NW * 8 + 8;               // TMEM columns of one stage's scales: W (each), then A
+    constexpr int SF0 = NW * MAX_T;                   // after the accumulators
+    constexpr int TMEM_COLS = GATED ? 512 : 256;      // a power of two >= SF0 + 2 * SF_COLS
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    Tail* tail = reinterpret_cast<Tail*>(smem + (size_t)g.stages * g.stage_bytes);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int tile = (int)(blockIdx.x / (unsigned)g.split);
+    const long long m0 = (long long)(tile / g.num_n_tiles) * MAX_T;   // t < MAX_T only when there is one row tile
+    const int n0 = (tile % g.num_n_tiles) * BN;
+    const int kb0 = (int)((long long)g.num_kb * rank / g.split), kb1 = (int)((long long)g.num_kb * (rank + 1) / g.split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < g.stages; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); }
+        mbar_init(&tail->done, 1);
+        tail->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_u32(&tail->tmem_base)), "r"((uint32_t)TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tail->tmem_base;
+    volatile int* abort_flag = &tail->abort_flag;
+    const int a_bytes = g.t * (BK / 2);
+
+    // stage: W (and Wu) codes, A codes, then the scales of W (and Wu) and of A
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            const uint8_t* sf_w = g.sw[0] + (long long)(n0 / mx::TILE_ROWS) * g.k_tiles * mx::TILE_BYTES;
+            const uint8_t* sf_u = GATED ? g.sw[1] + (long long)(n0 / mx::TILE_ROWS) * g.k_tiles * mx::TILE_BYTES : nullptr;
+            const uint8_t* sf_a = g.sa + (m0 / mx::TILE_ROWS) * g.k_tiles * mx::TILE_BYTES;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(&tail->empty[stage], phase ^ 1u, abort_flag, g.status, 151)) break;
+                uint8_t* s = smem + (size_t)stage * g.stage_bytes;
+                uint64_t* bar = &tail->full[stage];
+                const uint32_t sf = (uint32_t)min(2, g.k_tiles - 2 * kb) * mx::TILE_BYTES;
+                const long long sf_off = (long long)kb * SF_BYTES;
+                mbar_arrive_expect_tx(bar, (uint32_t)(NW * W_BYTES + a_bytes) + (NW + 1) * sf);
+                tma_load_2d(s, &map_w, bar, kb * (BK / 2), n0);
+                if (GATED) tma_load_2d(s + W_BYTES, &map_u, bar, kb * (BK / 2), n0);
+                tma_load_2d(s + NW * W_BYTES, &map_a, bar, kb * (BK / 2), (int)m0);
+                uint8_t* f = s + g.stage_bytes - (NW + 1) * SF_BYTES;
+                mx::bulk_load(f, sf_w + sf_off, sf, bar);
+                if (GATED) mx::bulk_load(f + SF_BYTES, sf_u + sf_off, sf, bar);
+                mx::bulk_load(f + NW * SF_BYTES, sf_a + sf_off, sf, bar);
+                if (++stage == g.stages) { stage = 0; phase ^= 1u; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 152);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t s = smem_u32(smem) + (uint32_t)(stage * g.stage_bytes);
+                const uint32_t f = s + (uint32_t)(g.stage_bytes - (NW + 1) * SF_BYTES);
+                const int steps = min(4, (g.K - kb * BK + 63) / 64);   // MMAs of 64 values; beyond K nothing is read
+                const uint32_t sf = tmem_base + (uint32_t)(SF0 + ((kb - kb0) & 1) * SF_COLS);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {                          // scale tiles of 128 values of K
+                    if (steps <= 2 * h) break;
+#pragma unroll
+                    for (int o = 0; o < NW + 1; ++o)
+                        mx::copy_scales(sf + (uint32_t)(o * 8 + h * 4), mx::make_scale_desc(f + (uint32_t)(o * SF_BYTES + h * mx::TILE_BYTES)));
+                }
+                const uint64_t adesc = make_smem_desc(s + NW * W_BYTES);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (k >= steps) break;
+                    const uint32_t idesc = g.idesc | mx::sf_bits(k & 1);
+#pragma unroll
+                    for (int o = 0; o < NW; ++o)
+                        mx::umma(tmem_base + (uint32_t)(o * MAX_T), make_smem_desc(s + o * W_BYTES) + (uint64_t)(k * 2), adesc + (uint64_t)(k * 2),
+                                 idesc, sf + (uint32_t)(o * 8 + (k >> 1) * 4), sf + (uint32_t)(NW * 8 + (k >> 1) * 4),
+                                 (uint32_t)(kb != kb0 || k != 0));
+                }
+                umma_commit(&tail->empty[stage]);
+                if (++stage == g.stages) { stage = 0; phase ^= 1u; }
+            }
+            if (ok) umma_commit(&tail->done);
+        }
+        __syncwarp();
+    }
+
+    const int quad = warp & 3;
+    const int nl = quad * 32 + lane;                                // feature within the tile
+    const int n = n0 + nl;
+    const int rows = (int)min((long long)g.t, g.M - m0);
+    bool ok = false;
+    if (warp >= 2) {
+        ok = mbar_wait(&tail->done, 0, abort_flag, g.status, 153);
+        tc_fence_after();
+    }
+    const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16);
+    float ba = 0.0f, bu = 0.0f;
+    if (warp >= 2 && n < g.N) {
+        if (g.bias[0]) ba = __ldg(g.bias[0] + n);
+        if (GATED && g.bias[1]) bu = __ldg(g.bias[1] + n);
+    }
+    if (g.split == 1) {
+        if (ok) {
+#pragma unroll 1
+            for (int c = 0; c < rows; c += 32) {
+                uint32_t a[32], u[32];
+                tmem_ld32(taddr + (uint32_t)c, a);
+                if (GATED) tmem_ld32(taddr + (uint32_t)(MAX_T + c), u);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (c + i < rows)
+                        store_value(g, m0 + c + i, n,
+                                    finish_value<GATED>(g, __uint_as_float(a[i]), GATED ? __uint_as_float(u[i]) : 0.0f, ba, bu));
+            }
+        }
+    } else {
+        // the partial tile [row][feature] in the stage buffers: all loads and MMAs of this CTA are complete
+        float* part = reinterpret_cast<float*>(smem);
+        if (ok) {
+#pragma unroll 1
+            for (int c = 0; c < rows; c += 16)
+#pragma unroll
+                for (int o = 0; o < NW; ++o) {
+                    uint32_t a[16];
+                    asm volatile(
+                        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]),
+                          "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])
+                        : "r"(taddr + (uint32_t)(o * MAX_T + c)));
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) part[(o * g.t + c + i) * BN + nl] = __uint_as_float(a[i]);
+                }
+        }
+        __syncthreads();
+        cluster_sync_all();
+        if (warp >= 2) {
+            const uint32_t base = smem_u32(part) + (uint32_t)(nl * 4);
+            for (int r = (int)rank; r < rows; r += g.split) {
+                float a = 0.0f, u = 0.0f;
+                for (int q = 0; q < g.split; ++q) {
+                    a += ld_cluster(base + (uint32_t)(r * BN * 4), (uint32_t)q);
+                    if (GATED) u += ld_cluster(base + (uint32_t)((g.t + r) * BN * 4), (uint32_t)q);
+                }
+                if (ok) store_value(g, m0 + r, n, finish_value<GATED>(g, a, u, ba, bu));
+            }
+        }
+        cluster_sync_all();      // nobody leaves while another rank reads its memory
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {           // copies in flight must land before the memory is given back
+        const uint64_t t0 = a4c_globaltimer();
+        while (a4c_globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem_base), "r"((uint32_t)TMEM_COLS) : "memory");
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn get_encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+    });
+    return fn;
+}
+
+// byte view of codes [rows, ceil(K / 2) bytes]; bytes outside read as zero
+bool make_map(CUtensorMap* map, const void* base, long long rows, int K, long long ld, int box_rows) {
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)((K + 1) / 2), (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(ld / 2)};
+    cuuint32_t box[2] = {(cuuint32_t)(BK / 2), (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool GATED>
+cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mw, const CUtensorMap& mu, const Args& g, unsigned grid, size_t smem,
+                   cudaStream_t s) {
+    static tc::SmemOptIn opt_in;
+    const cudaError_t e = opt_in.ensure(dense_mx_kernel<GATED>, SMEM_BUDGET + 16 * 1024);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)g.split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, dense_mx_kernel<GATED>, ma, mw, mu, g);
+}
+
+}  // namespace
+
+int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stream) {
+    const bool gated = d.wu != nullptr;
+    const int nw = gated ? 2 : 1;
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    Args g;
+    g.sa = d.sa; g.sw[0] = d.sw; g.sw[1] = d.su; g.bias[0] = d.bias; g.bias[1] = d.bias_u;
+    g.Y = d.y; g.ldy = d.ldy; g.ys = d.ys; g.y_across = mx::tiles_across(d.N);
+    g.M = d.M; g.N = d.N; g.K = d.K; g.k_tiles = (int)mx::tiles_across(d.K);
+    g.num_kb = (d.K + BK - 1) / BK;
+    g.out_kind = d.out_kind; g.act = d.act; g.status = status_word;
+    g.t = d.M >= MAX_T ? MAX_T : (int)((d.M + 15) / 16 * 16);
+    g.num_n_tiles = (d.N + BN - 1) / BN;
+    const long long tiles = (d.M + MAX_T - 1) / MAX_T * g.num_n_tiles;
+    if (tiles > 2147483647LL / MAX_SPLIT) return A4C_ERR_TOO_LARGE;
+    // split the reduction while a CTA per SM is not reached and every rank keeps a stage
+    g.split = 1;
+    while (g.split < MAX_SPLIT && tiles * g.split * 2 <= sms && g.split * 2 <= g.num_kb) g.split *= 2;
+    g.idesc = mx::make_idesc(BN, g.t);
+    g.stage_bytes = nw * W_BYTES + g.t * (BK / 2) + (nw + 1) * SF_BYTES;
+    const int need = (g.num_kb + g.split - 1) / g.split;
+    int stages = SMEM_BUDGET / g.stage_bytes;
+    if (stages > MAX_STAGES) stages = MAX_STAGES;
+    const int part_bytes = g.split > 1 ? nw * g.t * BN * 4 : 0;       // the partial tile lies over the stages
+    int least = (part_bytes + g.stage_bytes - 1) / g.stage_bytes;
+    if (need < stages) stages = need > least ? need : least;
+    g.stages = stages;
+    size_t smem = 1024 + (size_t)g.stages * g.stage_bytes + sizeof(Tail);
+    // More than half of an SM's shared memory, so that one CTA lives on an SM at a time: the ranks of a cluster wait for
+    // one another while they hold tensor memory, and two clusters that shared SMs could each wait for the other's.
+    if (smem < ONE_PER_SM) smem = ONE_PER_SM;
+    CUtensorMap ma, mw, mu;
+    if (!make_map(&ma, d.a, d.M, d.K, d.lda, g.t) || !make_map(&mw, d.w, d.N, d.K, d.ldw, BN) ||
+        !make_map(&mu, gated ? d.wu : d.w, d.N, d.K, gated ? d.ldu : d.ldw, BN))
+        return A4C_ERR_CUDA;
+    const unsigned grid = (unsigned)(tiles * g.split);
+    const cudaError_t err = gated ? launch<true>(ma, mw, mu, g, grid, smem, stream) : launch<false>(ma, mw, mu, g, grid, smem, stream);
+    return err == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
+}

@@ -66,6 +66,14 @@ SIGNATURES = {
     'a4c_bmm_f': (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64,
                           c_int, c_int, c_int, c_int, c_int, c_void_p]),
     'a4c_add_f': (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    'a4c_mx_scale_bytes': (c_int64, [c_int64, c_int64]),
+    'a4c_quantize_mx': (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p]),
+    'a4c_dequantize_mx': (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p]),
+    'a4c_dense_mx': (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64,
+                             c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),
+    'a4c_gated_dense_mx': (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_int, c_int, c_int,
+                                   c_void_p]),
     'a4c_add_layernorm_i8': (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
                                      c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     'a4c_dense_add_layernorm_supported': (c_int, [c_int64, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int, c_int,

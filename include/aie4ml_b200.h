@@ -235,6 +235,63 @@ A4C_API int a4c_add_f(const void* a, int64_t lda, const void* b, int64_t ldb, vo
               int64_t cols, int fdtype, void* stream);
 
 /*
+ * MXFP4: OCP microscaling with E2M1 elements.  (The reference has no block-scaled format; these entry points stand next to
+ * its float Dense, src/aie4ml/op_impls/families/matmul/resolver.py:110-127, for weights and activations held in 4 bits.)
+ *   value[r][c] = E2M1(code[r][c]) * 2^(scale[r][c / 32] - 127)      scale 255: the whole block is NaN
+ * E2M1 codes 0..7 are 0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 is the sign.
+ *   codes   two to a byte, even column in the low nibble; the row pitch is in ELEMENTS (codes) and a multiple of 32, the
+ *           base 16-byte aligned.  When the row length is odd, the last byte's high nibble must be 0.
+ *   scales  one byte per row and 32 columns, in tiles of 128 rows x 4 blocks = 512 bytes, a row group's tiles one after the
+ *           other: byte ((r / 128) * ceil(cols / 128) + b / 4) * 512 + (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 for row r,
+ *           block b.  a4c_mx_scale_bytes gives the size; the base is 16-byte aligned.  Blocks of a tile that lie beyond the
+ *           row's end must not be 255 (every entry point below writes them as 0); rows beyond the last one are not looked at.
+ * Errors as everywhere; A4C_ERR_ALIGNMENT for the rules above and for a float pointer not aligned to its element.
+ */
+A4C_API int64_t a4c_mx_scale_bytes(int64_t rows, int64_t cols);
+
+/*
+ * x [rows, cols] (fdtype 0 bfloat16, 1 float32, pitch ldx) -> codes (pitch ldc), scales.
+ *   scale = max(floor(log2(max |x| of the block)) - 2, -127) as 2^scale; a block holding a NaN or an infinity becomes NaN
+ *   code  = E2M1 nearest to x / 2^scale, ties to even, saturating at 6
+ * Exact in this sense: the result does not depend on the input's type.  Codes between cols and ldc are left as they are.
+ */
+A4C_API int a4c_quantize_mx(const void* x, int fdtype, int64_t ldx, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t rows,
+                            int64_t cols, void* stream);
+/* The values themselves: y [rows, cols] (fdtype 0 or 1, pitch ldy); bfloat16 holds every one of them exactly. */
+A4C_API int a4c_dequantize_mx(const uint8_t* codes, int64_t ldc, const uint8_t* scales, void* y, int fdtype, int64_t ldy,
+                              int64_t rows, int64_t cols, void* stream);
+
+/*
+ * Dense over MXFP4 operands:  Y = relu?( A . W + bias ), products accumulated in float32 on the tensor cores.
+ *   A [M, K] and Wt [N, K] (the weights TRANSPOSED, K contiguous) as above; bias float32 [N] or NULL
+ *   Y [M, N], pitch ldy: fdtype 0 bfloat16, 1 float32 (Y_scales NULL), or 3 MXFP4: codes in Y, scales in Y_scales, the float32
+ *   results quantised as by a4c_quantize_mx, ready to be the next layer's A
+ * Any M >= 0, K, N >= 1.  Y must not overlap an input.
+ */
+A4C_API int a4c_dense_mx(const uint8_t* A, int64_t lda, const uint8_t* A_scales, const uint8_t* Wt, int64_t ldw,
+                         const uint8_t* W_scales, const float* bias, void* Y, int fdtype, int64_t ldy, uint8_t* Y_scales,
+                         int64_t M, int K, int N, int relu, void* stream);
+
+/* Activations of a4c_gated_dense_mx */
+#define A4C_ACT_NONE 0
+#define A4C_ACT_RELU 1
+#define A4C_ACT_SILU 2       /* x / (1 + exp(-x)) */
+#define A4C_ACT_GELU 3       /* x (1 + erf(x / sqrt 2)) / 2 */
+#define A4C_ACT_GELU_TANH 4  /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+#define A4C_ACT_SIGMOID 5
+
+/*
+ * Gated Dense, the first half of a gated feed-forward block, in one kernel:
+ *   Y = act( A . Wg + bias_g ) * ( A . Wu + bias_u )
+ * Operands, outputs and rules as a4c_dense_mx, with two weight matrices [N, K]; either bias may be NULL.  With an MXFP4
+ * output the block's second half is a4c_dense_mx on Y.
+ */
+A4C_API int a4c_gated_dense_mx(const uint8_t* A, int64_t lda, const uint8_t* A_scales, const uint8_t* Wg, int64_t ldg,
+                               const uint8_t* Wg_scales, const uint8_t* Wu, int64_t ldu, const uint8_t* Wu_scales,
+                               const float* bias_g, const float* bias_u, void* Y, int fdtype, int64_t ldy, uint8_t* Y_scales,
+                               int64_t M, int K, int N, int activation, void* stream);
+
+/*
  * One attention head, fused:  out_b = srs( softmax_u8( srs(Q_b . K_b^T, qk_shift) ) . V_b, pv_shift )  for every
  * batch entry b.  The reference has no single kernel for this: it is the chain of its three kernels
  *   matmul_single::run with TRANSPOSE_B (src/aie4ml/templates/nnet_utils/matmul/matmul.cpp:32-118)
