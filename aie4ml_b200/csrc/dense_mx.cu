@@ -18,8 +18,6 @@
 // pipe takes both in issue order).  Every wait is bounded.
 #include <cuda.h>
 
-#include <mutex>
-
 #include "a4c_common.cuh"
 #include "a4c_kernels.h"
 #include "mx_common.cuh"
@@ -66,20 +64,9 @@ struct Args {
     int* status;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
-    uint32_t a;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mx::map_to_cta(local, rank)) : "memory");
     return v;
 }
 
@@ -137,7 +124,7 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank();
+    const uint32_t rank = mx::cluster_rank();
     const int tile = (int)(blockIdx.x / (unsigned)g.split);
     const long long m0 = (long long)(tile / g.num_n_tiles) * MAX_T;   // t < MAX_T only when there is one row tile
     const int n0 = (tile % g.num_n_tiles) * BN;
@@ -275,7 +262,7 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 }
         }
         __syncthreads();
-        cluster_sync_all();
+        mx::cluster_sync_all();
         if (warp >= 2) {
             const uint32_t base = smem_u32(part) + (uint32_t)(nl * 4);
             for (int r = (int)rank; r < rows; r += g.split) {
@@ -287,7 +274,7 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (ok) store_value(g, m0 + r, n, finish_value<GATED>(g, a, u, ba, bu));
             }
         }
-        cluster_sync_all();      // nobody leaves while another rank reads its memory
+        mx::cluster_sync_all();      // nobody leaves while another rank reads its memory
     }
 
     tc_fence_before();
@@ -301,36 +288,6 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem_base), "r"((uint32_t)TMEM_COLS) : "memory");
     }
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    return fn;
-}
-
-// byte view of codes [rows, ceil(K / 2) bytes]; bytes outside read as zero
-bool make_map(CUtensorMap* map, const void* base, long long rows, int K, long long ld, int box_rows) {
-    EncodeTiledFn fn = get_encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)((K + 1) / 2), (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)(ld / 2)};
-    cuuint32_t box[2] = {(cuuint32_t)(BK / 2), (cuuint32_t)box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <bool GATED>
@@ -362,6 +319,7 @@ int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stre
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (a4c_dense_mx_wide_wanted(d, sms)) return a4c_launch_dense_mx_wide(d, sms, status_word, stream);
     Args g;
     g.sa = d.sa; g.sw[0] = d.sw; g.sw[1] = d.su; g.bias[0] = d.bias; g.bias[1] = d.bias_u;
     g.Y = d.y; g.ldy = d.ldy; g.ys = d.ys; g.y_across = mx::tiles_across(d.N);
@@ -389,8 +347,8 @@ int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stre
     // one another while they hold tensor memory, and two clusters that shared SMs could each wait for the other's.
     if (smem < ONE_PER_SM) smem = ONE_PER_SM;
     CUtensorMap ma, mw, mu;
-    if (!make_map(&ma, d.a, d.M, d.K, d.lda, g.t) || !make_map(&mw, d.w, d.N, d.K, d.ldw, BN) ||
-        !make_map(&mu, gated ? d.wu : d.w, d.N, d.K, gated ? d.ldu : d.ldw, BN))
+    if (!mx::make_code_map(&ma, d.a, d.M, d.K, d.lda, g.t) || !mx::make_code_map(&mw, d.w, d.N, d.K, d.ldw, BN) ||
+        !mx::make_code_map(&mu, gated ? d.wu : d.w, d.N, d.K, gated ? d.ldu : d.ldw, BN))
         return A4C_ERR_CUDA;
     const unsigned grid = (unsigned)(tiles * g.split);
     const cudaError_t err = gated ? launch<true>(ma, mw, mu, g, grid, smem, stream) : launch<false>(ma, mw, mu, g, grid, smem, stream);

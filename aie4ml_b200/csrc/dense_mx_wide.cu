@@ -1,0 +1,381 @@
+// Dense and gated Dense over MXFP4 operands with many rows: a CTA pair (tcgen05 cta_group::2) per 256-row tile.
+// Same arithmetic as dense_mx.cu.
+//
+//   Dense: a tile is 256 rows x 256 features.  Gated: 256 rows x 128 features of both projections, the gate's 128 in
+//   accumulator columns 0-127 and the other's in 128-255, so that one thread holds both factors of an output.
+//
+// kind::mxf4 finishes a 256 x 256 x 256 step in 512 cycles; a single CTA on 128 x 256 would have to take in 48 KB of codes
+// in that time, the pair takes 32 KB per CTA: its own 128 rows of A and half of the weight rows (for the gated Dense one
+// CTA fetches the gate's rows, the other one the second projection's).  Scales go along as 2-tile boxes of a tensor map:
+// each CTA its own A rows', both CTAs all 256 weight rows'.
+//
+// Tensor memory: two accumulators of 256 columns and the scales of two stages (48 columns) are more than 512 columns, so the
+// accumulators overlap by 48 columns.  The epilogue empties those first and says so on a barrier of its own; the next
+// tile's MMAs wait for that and not for the whole tile.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-9 epilogue in two groups of four, each half of the columns.  A lane
+// holds one row, so an MXFP4 output block is 32 registers of one thread.  Every wait is bounded.
+#include <cuda.h>
+
+#include "a4c_common.cuh"
+#include "a4c_kernels.h"
+#include "mx_common.cuh"
+
+namespace {
+
+using namespace tc;
+
+constexpr int BM = 256, BM_CTA = 128;
+constexpr int BN = 256, BN_CTA = 128;         // weight rows per tile / staged per CTA
+constexpr int BK = 256;
+constexpr int CODE_BYTES = 128 * BK / 2;      // 128 rows of a stage's codes
+constexpr int SF_BYTES = 2 * mx::TILE_BYTES;  // and of its scales
+constexpr int STAGE_BYTES = 2 * CODE_BYTES + 3 * SF_BYTES;
+constexpr int STAGES = 6;
+constexpr int SF_COLS = 24;                   // A 8, weights 16
+constexpr int SF_SETS = 2;
+constexpr int TMEM_COLS = 512;
+constexpr int SF0 = TMEM_COLS - SF_SETS * SF_COLS;
+constexpr int ACC1 = SF0 - BN;                // second accumulator: columns ACC1 .. SF0
+constexpr int OVERLAP = BN - ACC1;
+constexpr int EPI_WARPS = 8;
+constexpr int NUM_THREADS = 64 + EPI_WARPS * 32;
+
+struct Tail {
+    uint64_t full[STAGES];
+    uint64_t empty[STAGES];
+    uint64_t tmem_full[2];
+    uint64_t tmem_empty[2];
+    uint64_t overlap_free[2];
+    uint32_t tmem_base;
+    volatile int abort_flag;
+};
+constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + sizeof(Tail);
+
+struct Args {
+    const float* bias[2];
+    void* Y; long long ldy;
+    uint8_t* ys; long long y_across;
+    long long M;
+    int K, N;
+    int num_kb;
+    int num_m_tiles, num_n_tiles;
+    int panel;                       // column tiles per panel of the tile order
+    int act;
+    uint32_t idesc;
+    int* status;
+};
+
+// column tile fastest inside a panel of weights that stays in the L2 while the row tiles stream past
+__device__ __forceinline__ void tile_coords(int tile, const Args& g, int& mt, int& nt) {
+    const int per_panel = g.num_m_tiles * g.panel;
+    const int pz = tile / per_panel, rem = tile - pz * per_panel;
+    const int width = min(g.panel, g.num_n_tiles - pz * g.panel);
+    mt = rem / width;
+    nt = pz * g.panel + (rem - mt * width);
+}
+
+// 32 finished neighbouring values of one row -> output
+template <int OUT>
+__device__ __forceinline__ void store32(const Args& g, long long row, int col, const float* v) {
+    const int left = g.N - col;
+    if (OUT == mx::KIND_BF16) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(g.Y) + row * g.ldy + col;
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = mx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        if (left >= 32 && ((uintptr_t)dst & 15u) == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) if (i < left) dst[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        }
+    } else if (OUT == mx::KIND_F32) {
+        float* dst = reinterpret_cast<float*>(g.Y) + row * g.ldy + col;
+        if (left >= 32 && ((uintptr_t)dst & 15u) == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) if (i < left) dst[i] = v[i];
+        }
+    } else {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        const uint32_t s = mx::scale_code(top);
+        const float inv = mx::inverse_scale(s == 255u ? 0u : s);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float q[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) q[k] = v[8 * i + k] * inv;
+            w[i] = s == 255u ? 0u : mx::pack_e2m1(q);
+        }
+        uint8_t* dst = reinterpret_cast<uint8_t*>(g.Y) + (row * g.ldy + col) / 2;
+        if (left >= 32) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else {
+            const int bytes = (left + 1) >> 1;
+#pragma unroll
+            for (int b = 0; b < 16; ++b) if (b < bytes) dst[b] = (uint8_t)(w[b >> 2] >> (8 * (b & 3)));
+        }
+        g.ys[mx::scale_offset(row, col >> 5, g.y_across)] = (uint8_t)s;
+    }
+}
+
+template <bool GATED, int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_sa,
+                     const __grid_constant__ CUtensorMap map_sw, const __grid_constant__ CUtensorMap map_su, Args g) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    Tail* tail = reinterpret_cast<Tail*>(smem + (size_t)STAGES * STAGE_BYTES);
+    constexpr int OUT_COLS = GATED ? 128 : 256;       // output features per tile
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = mx::cluster_rank();
+    const bool leader = rank == 0;
+    const int num_tiles = g.num_m_tiles * g.num_n_tiles;
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tail->tmem_full[a], 1);
+            mbar_init(&tail->tmem_empty[a], 2 * EPI_WARPS);
+            mbar_init(&tail->overlap_free[a], EPI_WARPS);      // one group of each CTA
+        }
+        tail->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_u32(&tail->tmem_base)), "r"((uint32_t)TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    mx::cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = tail->tmem_base;
+    volatile int* abort_flag = &tail->abort_flag;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+                int mt, nt;
+                tile_coords(tile, g, mt, nt);
+                const int m0 = mt * BM + (int)rank * BM_CTA;
+                const int n0 = nt * OUT_COLS;
+                const CUtensorMap* mw = GATED && rank ? &map_u : &map_w;
+                const int nw = GATED ? n0 : n0 + (int)rank * BN_CTA;
+                const int gw = n0 / mx::TILE_ROWS;
+                for (int kb = 0; kb < g.num_kb; ++kb) {
+                    ok = mbar_wait(&tail->empty[stage], phase ^ 1u, abort_flag, g.status, 161);
+                    if (!ok) break;
+                    uint8_t* s = smem + (size_t)stage * STAGE_BYTES;
+                    uint8_t* f = s + 2 * CODE_BYTES;
+                    const uint32_t bar = mx::map_to_cta(smem_u32(&tail->full[stage]), 0);
+                    if (leader) mbar_arrive_expect_tx(&tail->full[stage], 2 * STAGE_BYTES);
+                    mx::tma_load_2d_pair(s, &map_a, bar, kb * (BK / 2), m0);
+                    mx::tma_load_2d_pair(s + CODE_BYTES, mw, bar, kb * (BK / 2), nw);
+                    mx::tma_load_3d_pair(f, &map_sa, bar, 0, 2 * kb, m0 / mx::TILE_ROWS);
+                    mx::tma_load_3d_pair(f + SF_BYTES, &map_sw, bar, 0, 2 * kb, gw);
+                    mx::tma_load_3d_pair(f + 2 * SF_BYTES, GATED ? &map_su : &map_sw, bar, 0, 2 * kb, GATED ? gw : gw + 1);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (leader && lane == 0) {
+            int stage = 0, it = 0, step = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs, ++it) {
+                const int acc = it & 1;
+                ok = mbar_wait_spin(&tail->tmem_empty[acc], ((it >> 1) & 1) ^ 1u, abort_flag, g.status, 162);
+                if (ok && it > 0)
+                    ok = mbar_wait_spin(&tail->overlap_free[acc ^ 1], ((it - 1) >> 1) & 1, abort_flag, g.status, 163);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (uint32_t)(acc ? ACC1 : 0);
+                for (int kb = 0; kb < g.num_kb; ++kb, ++step) {
+                    ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 164);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t s = smem_u32(smem) + (uint32_t)(stage * STAGE_BYTES);
+                    const uint32_t f = s + 2 * CODE_BYTES;
+                    const int steps = min(4, (g.K - kb * BK + 63) / 64);
+                    // columns: A tile 0, A tile 1, weights tile 0 (8 columns: 256 rows), weights tile 1
+                    const uint32_t sf = tmem_base + (uint32_t)(SF0 + (step % SF_SETS) * SF_COLS);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (steps <= 2 * h) break;
+                        mx::copy_scales_pair(sf + (uint32_t)(h * 4), mx::make_scale_desc(f + (uint32_t)(h * mx::TILE_BYTES)));
+                        mx::copy_scales_pair(sf + (uint32_t)(8 + h * 8), mx::make_scale_desc(f + (uint32_t)(SF_BYTES + h * mx::TILE_BYTES)));
+                        mx::copy_scales_pair(sf + (uint32_t)(12 + h * 8), mx::make_scale_desc(f + (uint32_t)(2 * SF_BYTES + h * mx::TILE_BYTES)));
+                    }
+                    const uint64_t adesc = make_smem_desc(s), bdesc = make_smem_desc(s + CODE_BYTES);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (k >= steps) break;
+                        mx::umma_pair(d_tmem, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), g.idesc | mx::sf_bits(k & 1),
+                                      sf + (uint32_t)((k >> 1) * 4), sf + (uint32_t)(8 + (k >> 1) * 8), (uint32_t)((kb | k) != 0));
+                    }
+                    mx::commit_pair(smem_u32(&tail->empty[stage]));
+                    mx::commit_pair(mx::map_to_cta(smem_u32(&tail->empty[stage]), 1));
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                mx::commit_pair(smem_u32(&tail->tmem_full[acc]));
+                mx::commit_pair(mx::map_to_cta(smem_u32(&tail->tmem_full[acc]), 1));
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quad = warp & 3;
+        const int grp = (warp - 2) >> 2;
+        const uint32_t lane_base = tmem_base + ((uint32_t)(quad * 32) << 16);
+        constexpr int CHUNKS = GATED ? 2 : 4;                  // pieces of 32 output columns per group
+        constexpr int GROUP_COLS = CHUNKS * 32;
+        // pieces until the overlapping columns are in registers (they are the last of accumulator 0, the first of 1; for the
+        // gated Dense the second factor's last columns and the gate's first ones)
+        constexpr int OVERLAP_CHUNKS = (OVERLAP + 31) / 32;
+        static_assert(OVERLAP_CHUNKS <= CHUNKS, "the overlap lies within one group's columns");
+        int it = 0;
+        bool ok = true;
+        for (int tile = pair; tile < num_tiles; tile += num_pairs, ++it) {
+            int mt, nt;
+            tile_coords(tile, g, mt, nt);
+            const int acc = it & 1;
+            const long long row = (long long)mt * BM + (int)rank * BM_CTA + quad * 32 + lane;
+            const int n0 = nt * OUT_COLS;
+            if (ok) ok = mbar_wait(&tail->tmem_full[acc], (it >> 1) & 1, abort_flag, g.status, 165);
+            if (!ok) continue;
+            tc_fence_after();
+            const uint32_t taddr = lane_base + (uint32_t)(acc ? ACC1 : 0);
+            const bool holds_overlap = acc ? grp == 0 : grp == 1;
+            const bool down = acc == 0 && grp == 1;            // from the top, where accumulator 0 overlaps
+#pragma unroll 1
+            for (int j = 0; j < CHUNKS; ++j) {
+                const int c = grp * GROUP_COLS + 32 * (down ? CHUNKS - 1 - j : j);
+                uint32_t a[32], u[32];
+                tmem_ld32_async(taddr + (uint32_t)c, a);
+                if (GATED) { tmem_ld32_async(taddr + (uint32_t)(128 + c), u); tmem_ld_wait32(u); }
+                tmem_ld_wait32(a);
+                const bool last = j == CHUNKS - 1, over = holds_overlap && j == OVERLAP_CHUNKS - 1;
+                if (last || over) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (over) mx::mbar_arrive_cluster(mx::map_to_cta(smem_u32(&tail->overlap_free[acc]), 0));
+                        if (last) mx::mbar_arrive_cluster(mx::map_to_cta(smem_u32(&tail->tmem_empty[acc]), 0));
+                    }
+                }
+                const int col = n0 + c;
+                if (col < g.N) {
+                    float v[32];
+                    const bool whole = col + 32 <= g.N;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(a[i]);
+                    if (g.bias[0]) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] += whole || col + i < g.N ? __ldg(g.bias[0] + col + i) : 0.0f;
+                    }
+                    if (GATED) {
+                        float w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(u[i]);
+                        if (g.bias[1]) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) w[i] += whole || col + i < g.N ? __ldg(g.bias[1] + col + i) : 0.0f;
+                        }
+                        mx::activate32(v, g.act);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] *= w[i];
+                    } else if (g.act == mx::ACT_RELU) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+                    }
+                    if (OUT == mx::KIND_MX && !whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) if (col + i >= g.N) v[i] = 0.0f;
+                    }
+                    if (row < g.M) store32<OUT>(g, row, col, v);
+                } else if (OUT == mx::KIND_MX && row < g.M && (col >> 5) < (int)g.y_across * mx::TILE_BLOCKS) {
+                    g.ys[mx::scale_offset(row, col >> 5, g.y_across)] = 0;       // block beyond the row's end
+                }
+            }
+        }
+    }
+
+    __syncthreads();
+    if (*abort_flag) {
+        const uint64_t t0 = a4c_globaltimer();
+        while (a4c_globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    tc_fence_before();
+    mx::cluster_sync_all();
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem_base), "r"((uint32_t)TMEM_COLS) : "memory");
+}
+
+template <bool GATED, int OUT>
+cudaError_t launch(const CUtensorMap* m, const Args& g, int grid, cudaStream_t s) {
+    static tc::SmemOptIn opt_in;
+    const cudaError_t e = opt_in.ensure(dense_mx_wide_kernel<GATED, OUT>, SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    dense_mx_wide_kernel<GATED, OUT><<<grid, NUM_THREADS, SMEM_BYTES, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], g);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+// Tiles of the pair kernel; below about a wave of pairs the smaller tiles of dense_mx.cu spread better over the SMs.
+bool a4c_dense_mx_wide_wanted(const A4cMxDense& d, int sms) {
+    const long long cols = d.wu != nullptr ? 128 : 256;
+    const long long tiles = ((d.M + BM - 1) / BM) * ((d.N + cols - 1) / cols);
+    return tiles * 2 >= sms / 2 && d.M > 128;
+}
+
+int a4c_launch_dense_mx_wide(const A4cMxDense& d, int sms, int* status_word, cudaStream_t stream) {
+    const bool gated = d.wu != nullptr;
+    Args g;
+    g.bias[0] = d.bias; g.bias[1] = d.bias_u; g.Y = d.y; g.ldy = d.ldy; g.ys = d.ys; g.y_across = mx::tiles_across(d.N);
+    g.M = d.M; g.K = d.K; g.N = d.N; g.act = d.act; g.status = status_word;
+    g.num_kb = (d.K + BK - 1) / BK;
+    const int cols = gated ? 128 : 256;
+    const long long mt = (d.M + BM - 1) / BM, nt = (d.N + cols - 1) / cols;
+    if (mt * nt > 2147483647LL - 65536) return A4C_ERR_TOO_LARGE;
+    g.num_m_tiles = (int)mt; g.num_n_tiles = (int)nt;
+    const long long tile_bytes = (long long)BN * g.num_kb * (BK / 2);
+    long long panel = (32LL << 20) / tile_bytes;
+    g.panel = (int)(panel < 1 ? 1 : (panel > nt ? nt : panel));
+    g.idesc = mx::make_idesc(BM, BN);
+    CUtensorMap m[6];
+    if (!mx::make_code_map(&m[0], d.a, d.M, d.K, d.lda, BM_CTA) || !mx::make_code_map(&m[1], d.w, d.N, d.K, d.ldw, BN_CTA) ||
+        !mx::make_scale_map(&m[3], d.sa, d.M, d.K) || !mx::make_scale_map(&m[4], d.sw, d.N, d.K))
+        return A4C_ERR_CUDA;
+    m[2] = m[1]; m[5] = m[4];
+    if (gated && (!mx::make_code_map(&m[2], d.wu, d.N, d.K, d.ldu, BN_CTA) || !mx::make_scale_map(&m[5], d.su, d.N, d.K))) return A4C_ERR_CUDA;
+    const long long pairs = mt * nt < sms / 2 ? mt * nt : sms / 2;
+    const int grid = (int)pairs * 2;
+    cudaError_t err;
+    if (gated)
+        err = d.out_kind == mx::KIND_BF16 ? launch<true, mx::KIND_BF16>(m, g, grid, stream)
+              : d.out_kind == mx::KIND_F32 ? launch<true, mx::KIND_F32>(m, g, grid, stream) : launch<true, mx::KIND_MX>(m, g, grid, stream);
+    else
+        err = d.out_kind == mx::KIND_BF16 ? launch<false, mx::KIND_BF16>(m, g, grid, stream)
+              : d.out_kind == mx::KIND_F32 ? launch<false, mx::KIND_F32>(m, g, grid, stream) : launch<false, mx::KIND_MX>(m, g, grid, stream);
+    return err == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
+}

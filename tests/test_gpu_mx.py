@@ -173,6 +173,10 @@ SHAPES = [(1, 1, 1), (1, 32, 16), (3, 33, 5), (1, 4096, 200), (16, 64, 128), (17
           (128, 512, 384), (129, 1000, 777), (200, 130, 1024), (256, 2048, 256), (333, 1000, 65), (385, 4096, 640)]
 
 
+# enough tiles of 256 x 256 (and of 256 x 128 pairs of features) that a CTA pair works through several
+WIDE = [(1030, 300, 2600), (2600, 64, 5000), (3001, 520, 4500), (300, 257, 9700)]
+
+
 def run_dense(lib, a, w, bias, out, relu):
     lib.check(lib.load().a4c_dense_mx(*a.args, *w.args, bias.data_ptr() if bias is not None else None, *out.args, a.rows, a.cols, w.rows, relu,
                                       stream()), 'dense')
@@ -183,7 +187,7 @@ def exact_bias(rng, n):
     return rng.integers(-1024, 1025, n) / 16.0
 
 
-@pytest.mark.parametrize('m,k,n', SHAPES)
+@pytest.mark.parametrize('m,k,n', SHAPES + WIDE)
 @pytest.mark.parametrize('kind', ['bf16', 'f32', 'mx'])
 def test_dense_exact(lib, m, k, n, kind):
     t = torch()
@@ -199,7 +203,7 @@ def test_dense_exact(lib, m, k, n, kind):
     got = out.get()
     assert lib.device_status() == 0
     if kind == 'mx':
-        codes, scales = R.quantize(want)
+        codes, scales = (np.concatenate(p) for p in zip(*(R.quantize(want[i:i + 512]) for i in range(0, m, 512))))
         assert np.array_equal(got[1], scales)
         assert np.array_equal(R.values(*got), R.values(codes, scales))      # a zero's sign is free
     else:
@@ -266,7 +270,7 @@ def dev32(x):
     return None if x is None else torch().from_numpy(np.asarray(x, dtype=np.float32)).cuda()
 
 
-@pytest.mark.parametrize('m,k,n', SHAPES)
+@pytest.mark.parametrize('m,k,n', SHAPES + WIDE)
 @pytest.mark.parametrize('kind', ['bf16', 'f32', 'mx'])
 def test_gated_exact(lib, m, k, n, kind):
     rng = np.random.default_rng(m * 7907 + k * 37 + n)
@@ -281,7 +285,7 @@ def test_gated_exact(lib, m, k, n, kind):
     got = out.get()
     assert lib.device_status() == 0
     if kind == 'mx':
-        codes, scales = R.quantize(want)
+        codes, scales = (np.concatenate(p) for p in zip(*(R.quantize(want[i:i + 512]) for i in range(0, m, 512))))
         assert np.array_equal(got[1], scales)
         assert np.array_equal(R.values(*got), R.values(codes, scales))
     else:
