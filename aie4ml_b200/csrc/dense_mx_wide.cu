@@ -13,8 +13,14 @@
 // accumulators overlap by 48 columns.  The epilogue empties those first and says so on a barrier of its own; the next
 // tile's MMAs wait for that and not for the whole tile.
 //
-// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-9 epilogue in two groups of four, each half of the columns.  A lane
-// holds one row, so an MXFP4 output block is 32 registers of one thread.  Every wait is bounded.
+// The scale copies (tcgen05.cp) have a warp of their own, one stage ahead of the MMAs and tied to them by barriers: issued
+// by the MMA thread they run in turn with the MMAs, six copies of a stage costing 0.22 us on top of its 0.40 us of MMAs
+// (4096 x 16384 x 8192: 303 us; spread out between the MMAs 346 us; from their own warp 240 us, no copies at all 205 us).
+//
+// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-9 epilogue in two groups of four, each half of the columns, 10 scale
+// copies (leader CTA).  A lane holds one row, so an MXFP4 output block is 32 registers of one thread; rows go out through a
+// swizzled patch of shared memory per warp and TMA stores (directly from registers every 16 bytes of a row were an L2
+// request of their own).  Every wait is bounded.
 #include <cuda.h>
 
 #include "a4c_common.cuh"
@@ -31,7 +37,7 @@ constexpr int BK = 256;
 constexpr int CODE_BYTES = 128 * BK / 2;      // 128 rows of a stage's codes
 constexpr int SF_BYTES = 2 * mx::TILE_BYTES;  // and of its scales
 constexpr int STAGE_BYTES = 2 * CODE_BYTES + 3 * SF_BYTES;
-constexpr int STAGES = 6;
+constexpr int STAGES = 5;
 constexpr int SF_COLS = 24;                   // A 8, weights 16
 constexpr int SF_SETS = 2;
 constexpr int TMEM_COLS = 512;
@@ -39,7 +45,8 @@ constexpr int SF0 = TMEM_COLS - SF_SETS * SF_COLS;
 constexpr int ACC1 = SF0 - BN;                // second accumulator: columns ACC1 .. SF0
 constexpr int OVERLAP = BN - ACC1;
 constexpr int EPI_WARPS = 8;
-constexpr int NUM_THREADS = 64 + EPI_WARPS * 32;
+constexpr int NUM_THREADS = 96 + EPI_WARPS * 32;
+constexpr int PATCH_BYTES = 32 * 128;           // per epilogue warp: 32 rows of a TMA store's box
 
 struct Tail {
     uint64_t full[STAGES];
@@ -47,10 +54,11 @@ struct Tail {
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
     uint64_t overlap_free[2];
+    uint64_t sf_full[SF_SETS];
     uint32_t tmem_base;
     volatile int abort_flag;
 };
-constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + sizeof(Tail);
+constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * PATCH_BYTES + sizeof(Tail);
 
 struct Args {
     const float* bias[2];
@@ -62,6 +70,7 @@ struct Args {
     int num_m_tiles, num_n_tiles;
     int panel;                       // column tiles per panel of the tile order
     int act;
+    int tma_store;                   // the output's base and pitch are multiples of 16 bytes
     uint32_t idesc;
     int* status;
 };
@@ -75,64 +84,77 @@ __device__ __forceinline__ void tile_coords(int tile, const Args& g, int& mt, in
     nt = pz * g.panel + (rem - mt * width);
 }
 
-// 32 finished neighbouring values of one row -> output
+// 32 finished neighbouring values of one row -> words of the output type (16 bf16, 32 f32, 4 MXFP4) and its scale
 template <int OUT>
-__device__ __forceinline__ void store32(const Args& g, long long row, int col, const float* v) {
+__device__ __forceinline__ uint32_t to_words(const float* v, uint32_t* w) {
+    if (OUT == mx::KIND_BF16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = mx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        return 0;
+    }
+    if (OUT == mx::KIND_F32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
+        return 0;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    const uint32_t s = mx::scale_code(top);
+    const float inv = mx::inverse_scale(s == 255u ? 0u : s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[k] = v[8 * i + k] * inv;
+        w[i] = s == 255u ? 0u : mx::pack_e2m1(q);
+    }
+    return s;
+}
+
+template <int OUT> struct Words { static constexpr int value = OUT == mx::KIND_BF16 ? 16 : OUT == mx::KIND_F32 ? 32 : 4; };
+
+// straight from registers: for outputs that a tensor map cannot describe, and for boxes that reach beyond the row's end (a TMA
+// store there wrote up to the next 16 bytes of the row)
+template <int OUT>
+__device__ __forceinline__ void store_direct(const Args& g, long long row, int col, const uint32_t* w) {
     const int left = g.N - col;
     if (OUT == mx::KIND_BF16) {
         uint16_t* dst = reinterpret_cast<uint16_t*>(g.Y) + row * g.ldy + col;
-        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = mx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
-        if (left >= 32 && ((uintptr_t)dst & 15u) == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) if (i < left) dst[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-        }
+        for (int i = 0; i < 32; ++i) if (i < left) dst[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
     } else if (OUT == mx::KIND_F32) {
-        float* dst = reinterpret_cast<float*>(g.Y) + row * g.ldy + col;
-        if (left >= 32 && ((uintptr_t)dst & 15u) == 0) {
+        uint32_t* dst = reinterpret_cast<uint32_t*>(g.Y) + row * g.ldy + col;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) if (i < left) dst[i] = v[i];
-        }
+        for (int i = 0; i < 32; ++i) if (i < left) dst[i] = w[i];
     } else {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-        const uint32_t s = mx::scale_code(top);
-        const float inv = mx::inverse_scale(s == 255u ? 0u : s);
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float q[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) q[k] = v[8 * i + k] * inv;
-            w[i] = s == 255u ? 0u : mx::pack_e2m1(q);
-        }
         uint8_t* dst = reinterpret_cast<uint8_t*>(g.Y) + (row * g.ldy + col) / 2;
+        const int bytes = (left + 1) >> 1;
         if (left >= 32) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         else {
-            const int bytes = (left + 1) >> 1;
 #pragma unroll
             for (int b = 0; b < 16; ++b) if (b < bytes) dst[b] = (uint8_t)(w[b >> 2] >> (8 * (b & 3)));
         }
-        g.ys[mx::scale_offset(row, col >> 5, g.y_across)] = (uint8_t)s;
     }
 }
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                 :: "l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 template <bool GATED, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_sa,
-                     const __grid_constant__ CUtensorMap map_sw, const __grid_constant__ CUtensorMap map_su, Args g) {
+                     const __grid_constant__ CUtensorMap map_sw, const __grid_constant__ CUtensorMap map_su,
+                     const __grid_constant__ CUtensorMap map_y, Args g) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    Tail* tail = reinterpret_cast<Tail*>(smem + (size_t)STAGES * STAGE_BYTES);
+    uint8_t* patches = smem + (size_t)STAGES * STAGE_BYTES;
+    Tail* tail = reinterpret_cast<Tail*>(patches + EPI_WARPS * PATCH_BYTES);
     constexpr int OUT_COLS = GATED ? 128 : 256;       // output features per tile
 
     const int warp = threadIdx.x >> 5;
@@ -149,6 +171,7 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             mbar_init(&tail->tmem_empty[a], 2 * EPI_WARPS);
             mbar_init(&tail->overlap_free[a], EPI_WARPS);      // one group of each CTA
         }
+        for (int i = 0; i < SF_SETS; ++i) mbar_init(&tail->sf_full[i], 1);
         tail->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -208,21 +231,13 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(acc ? ACC1 : 0);
                 for (int kb = 0; kb < g.num_kb; ++kb, ++step) {
-                    ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 164);
+                    ok = mbar_wait(&tail->sf_full[step % SF_SETS], (step / SF_SETS) & 1, abort_flag, g.status, 164) &&
+                         mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 164);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t s = smem_u32(smem) + (uint32_t)(stage * STAGE_BYTES);
-                    const uint32_t f = s + 2 * CODE_BYTES;
                     const int steps = min(4, (g.K - kb * BK + 63) / 64);
-                    // columns: A tile 0, A tile 1, weights tile 0 (8 columns: 256 rows), weights tile 1
                     const uint32_t sf = tmem_base + (uint32_t)(SF0 + (step % SF_SETS) * SF_COLS);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (steps <= 2 * h) break;
-                        mx::copy_scales_pair(sf + (uint32_t)(h * 4), mx::make_scale_desc(f + (uint32_t)(h * mx::TILE_BYTES)));
-                        mx::copy_scales_pair(sf + (uint32_t)(8 + h * 8), mx::make_scale_desc(f + (uint32_t)(SF_BYTES + h * mx::TILE_BYTES)));
-                        mx::copy_scales_pair(sf + (uint32_t)(12 + h * 8), mx::make_scale_desc(f + (uint32_t)(2 * SF_BYTES + h * mx::TILE_BYTES)));
-                    }
                     const uint64_t adesc = make_smem_desc(s), bdesc = make_smem_desc(s + CODE_BYTES);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -240,6 +255,35 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             }
         }
         __syncwarp();
+    } else if (warp == 10) {
+        if (leader && lane == 0) {
+            const int total = ((num_tiles - pair + num_pairs - 1) / num_pairs) * g.num_kb;
+            int stage = 0, kb = 0;
+            uint32_t phase = 0;
+            for (int step = 0; step < total; ++step) {
+                bool ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 166);
+                if (ok && step >= SF_SETS) {           // the MMAs that read this set's last contents are done
+                    const int old = step - SF_SETS;
+                    ok = mbar_wait(&tail->empty[old % STAGES], (old / STAGES) & 1, abort_flag, g.status, 167);
+                }
+                if (!ok) break;
+                tc_fence_after();
+                // columns of a set: A tile 0, A tile 1, weights tile 0 (8 columns: 256 rows), weights tile 1
+                const uint32_t f = smem_u32(smem) + (uint32_t)(stage * STAGE_BYTES + 2 * CODE_BYTES);
+                const uint32_t sf = tmem_base + (uint32_t)(SF0 + (step % SF_SETS) * SF_COLS);
+                const int halves = g.K - kb * BK > 128 ? 2 : 1;
+                for (int h = 0; h < halves; ++h) {
+                    const uint32_t t = (uint32_t)(h * mx::TILE_BYTES);
+                    mx::copy_scales_pair(sf + (uint32_t)(h * 4), mx::make_scale_desc(f + t));
+                    mx::copy_scales_pair(sf + (uint32_t)(8 + h * 8), mx::make_scale_desc(f + SF_BYTES + t));
+                    mx::copy_scales_pair(sf + (uint32_t)(12 + h * 8), mx::make_scale_desc(f + 2 * SF_BYTES + t));
+                }
+                mx::commit_pair(smem_u32(&tail->sf_full[step % SF_SETS]));
+                if (++kb == g.num_kb) kb = 0;
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+        }
+        __syncwarp();
     } else {
         const int quad = warp & 3;
         const int grp = (warp - 2) >> 2;
@@ -250,13 +294,16 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         // gated Dense the second factor's last columns and the gate's first ones)
         constexpr int OVERLAP_CHUNKS = (OVERLAP + 31) / 32;
         static_assert(OVERLAP_CHUNKS <= CHUNKS, "the overlap lies within one group's columns");
+        constexpr int WORDS = Words<OUT>::value;
+        constexpr int PER_BOX = OUT == mx::KIND_F32 ? 1 : 2;   // pieces per TMA store: 128 bytes of bf16 or f32, 32 of MXFP4
+        uint8_t* patch = patches + (warp - 2) * PATCH_BYTES;
         int it = 0;
         bool ok = true;
         for (int tile = pair; tile < num_tiles; tile += num_pairs, ++it) {
             int mt, nt;
             tile_coords(tile, g, mt, nt);
             const int acc = it & 1;
-            const long long row = (long long)mt * BM + (int)rank * BM_CTA + quad * 32 + lane;
+            const long long row0 = (long long)mt * BM + (int)rank * BM_CTA + quad * 32, row = row0 + lane;
             const int n0 = nt * OUT_COLS;
             if (ok) ok = mbar_wait(&tail->tmem_full[acc], (it >> 1) & 1, abort_flag, g.status, 165);
             if (!ok) continue;
@@ -281,40 +328,65 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     }
                 }
                 const int col = n0 + c;
-                if (col < g.N) {
-                    float v[32];
-                    const bool whole = col + 32 <= g.N;
+                if (row0 >= g.M) continue;
+                float v[32];
+                const bool whole = col + 32 <= g.N;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(a[i]);
-                    if (g.bias[0]) {
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(a[i]);
+                if (g.bias[0]) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] += whole || col + i < g.N ? __ldg(g.bias[0] + col + i) : 0.0f;
+                    for (int i = 0; i < 32; ++i) v[i] += whole || col + i < g.N ? __ldg(g.bias[0] + col + i) : 0.0f;
+                }
+                if (GATED) {
+                    float w[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(u[i]);
+                    if (g.bias[1]) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i] += whole || col + i < g.N ? __ldg(g.bias[1] + col + i) : 0.0f;
                     }
-                    if (GATED) {
-                        float w[32];
+                    mx::activate32(v, g.act);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(u[i]);
-                        if (g.bias[1]) {
+                    for (int i = 0; i < 32; ++i) v[i] *= w[i];
+                } else if (g.act == mx::ACT_RELU) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) w[i] += whole || col + i < g.N ? __ldg(g.bias[1] + col + i) : 0.0f;
-                        }
-                        mx::activate32(v, g.act);
+                    for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+                }
+                if (OUT == mx::KIND_MX && !whole) {            // (the same for a block wholly beyond the row's end: scale 0)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] *= w[i];
-                    } else if (g.act == mx::ACT_RELU) {
+                    for (int i = 0; i < 32; ++i) if (col + i >= g.N) v[i] = 0.0f;
+                }
+                uint32_t w[WORDS];
+                const uint32_t scale = to_words<OUT>(v, w);
+                if (OUT == mx::KIND_MX && row < g.M && (col >> 5) < (int)g.y_across * mx::TILE_BLOCKS)
+                    g.ys[mx::scale_offset(row, col >> 5, g.y_across)] = (uint8_t)scale;
+                const int col0 = n0 + (c & ~(32 * PER_BOX - 1));
+                if (!g.tma_store || col0 + 32 * PER_BOX > g.N) {
+                    if (row < g.M && col < g.N) store_direct<OUT>(g, row, col, w);
+                    continue;
+                }
+                const int half = PER_BOX == 2 ? (c >> 5) & 1 : 0;              // which half of the box's columns
+                if (j % PER_BOX == 0) {                                         // the patch's last store has been read
+                    if (lane == 0) tma_store_wait_read();
+                    __syncwarp();
+                }
+                if (OUT == mx::KIND_MX) {
+                    *reinterpret_cast<uint4*>(patch + lane * 32 + half * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
-                    }
-                    if (OUT == mx::KIND_MX && !whole) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) if (col + i >= g.N) v[i] = 0.0f;
-                    }
-                    if (row < g.M) store32<OUT>(g, row, col, v);
-                } else if (OUT == mx::KIND_MX && row < g.M && (col >> 5) < (int)g.y_across * mx::TILE_BLOCKS) {
-                    g.ys[mx::scale_offset(row, col >> 5, g.y_across)] = 0;       // block beyond the row's end
+                    for (int i = 0; i < WORDS / 4; ++i)                         // 128-byte swizzle: 16-byte piece p of row r at p ^ (r & 7)
+                        *reinterpret_cast<uint4*>(patch + lane * 128 + (((half * 4 + i) ^ (lane & 7)) << 4)) =
+                            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
+                if (j % PER_BOX == PER_BOX - 1) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0)
+                        tma_store_2d(&map_y, patch, OUT == mx::KIND_MX ? col0 / 2 : col0, (int)row0);
                 }
             }
         }
+        if (lane == 0) tma_store_wait_read();      // the patch outlives its last store
     }
 
     __syncthreads();
@@ -335,7 +407,7 @@ cudaError_t launch(const CUtensorMap* m, const Args& g, int grid, cudaStream_t s
     static tc::SmemOptIn opt_in;
     const cudaError_t e = opt_in.ensure(dense_mx_wide_kernel<GATED, OUT>, SMEM_BYTES);
     if (e != cudaSuccess) return e;
-    dense_mx_wide_kernel<GATED, OUT><<<grid, NUM_THREADS, SMEM_BYTES, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], g);
+    dense_mx_wide_kernel<GATED, OUT><<<grid, NUM_THREADS, SMEM_BYTES, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], g);
     return cudaGetLastError();
 }
 
@@ -362,12 +434,16 @@ int a4c_launch_dense_mx_wide(const A4cMxDense& d, int sms, int* status_word, cud
     long long panel = (32LL << 20) / tile_bytes;
     g.panel = (int)(panel < 1 ? 1 : (panel > nt ? nt : panel));
     g.idesc = mx::make_idesc(BM, BN);
-    CUtensorMap m[6];
+    CUtensorMap m[7];
     if (!mx::make_code_map(&m[0], d.a, d.M, d.K, d.lda, BM_CTA) || !mx::make_code_map(&m[1], d.w, d.N, d.K, d.ldw, BN_CTA) ||
         !mx::make_scale_map(&m[3], d.sa, d.M, d.K) || !mx::make_scale_map(&m[4], d.sw, d.N, d.K))
         return A4C_ERR_CUDA;
     m[2] = m[1]; m[5] = m[4];
     if (gated && (!mx::make_code_map(&m[2], d.wu, d.N, d.K, d.ldu, BN_CTA) || !mx::make_scale_map(&m[5], d.su, d.N, d.K))) return A4C_ERR_CUDA;
+    const int esz = d.out_kind == mx::KIND_BF16 ? 2 : 4;
+    g.tma_store = d.out_kind == mx::KIND_MX || (((uintptr_t)d.y & 15u) == 0 && (d.ldy * esz) % 16 == 0);
+    m[6] = m[0];
+    if (g.tma_store && !mx::make_out_map(&m[6], d.y, d.out_kind, d.M, d.N, d.ldy)) return A4C_ERR_CUDA;
     const long long pairs = mt * nt < sms / 2 ? mt * nt : sms / 2;
     const int grid = (int)pairs * 2;
     cudaError_t err;

@@ -196,6 +196,21 @@ inline bool make_scale_map(CUtensorMap* map, const void* base, long long rows, i
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// an output [rows, cols] for TMA stores of 32 rows: 128 bytes of bf16 or f32 (128-byte swizzle), 32 bytes (64 codes) of MXFP4
+inline bool make_out_map(CUtensorMap* map, void* base, int kind, long long rows, int cols, long long ld) {
+    const EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const bool codes = kind == KIND_MX;
+    const int esz = kind == KIND_F32 ? 4 : 2;
+    cuuint64_t dims[2] = {(cuuint64_t)(codes ? (cols + 1) / 2 : cols), (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(codes ? ld / 2 : ld * esz)};
+    cuuint32_t box[2] = {(cuuint32_t)(codes ? 32 : 128 / esz), 32};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(map, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : kind == KIND_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+              2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 // ---- activations of the gated Dense -------------------------------------------------------------
 constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_SIGMOID = 5, ACT_COUNT = 6;

@@ -73,7 +73,8 @@ class Out:
     def __init__(self, kind, rows, cols):
         t = torch()
         self.kind, self.rows, self.cols = kind, rows, cols
-        self.ld = up(cols) + 32 if kind == 'mx' else cols + 3
+        # float outputs: every third has a pitch that no wide store can use
+        self.ld = up(cols) + 32 if kind == 'mx' else cols + 3 if (rows + cols) % 3 == 0 else up(cols, 8) + 8
         width = self.ld // 2 if kind == 'mx' else self.ld
         dtype = {'mx': t.uint8, 'bf16': t.bfloat16, 'f32': t.float32}[kind]
         self.buf = t.full((rows + 2, width), 0x55 if kind == 'mx' else -7.0, dtype=dtype, device='cuda')
@@ -81,7 +82,7 @@ class Out:
 
     @property
     def args(self):
-        return self.buf[1].data_ptr(), F[self.kind], self.ld, self.scales.data_ptr() if self.scales is not None else None
+        return self.buf[1:].data_ptr(), F[self.kind], self.ld, self.scales.data_ptr() if self.scales is not None else None
 
     def get(self):
         torch().cuda.synchronize()
