@@ -84,9 +84,12 @@ __device__ __forceinline__ void tile_coords(int tile, const Args& g, int& mt, in
     nt = pz * g.panel + (rem - mt * width);
 }
 
-// 32 finished neighbouring values of one row -> words of the output type (16 bf16, 32 f32, 4 MXFP4) and its scale
+// 32 finished neighbouring values of one row (as pairs) -> words of the output type (16 bf16, 32 f32, 4 MXFP4) and its scale
 template <int OUT>
-__device__ __forceinline__ uint32_t to_words(const float* v, uint32_t* w) {
+__device__ __forceinline__ uint32_t to_words(const mx::f2* p, uint32_t* w) {
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx::unpack2(p[i], v[2 * i], v[2 * i + 1]);
     if (OUT == mx::KIND_BF16) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i] = mx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
@@ -97,19 +100,35 @@ __device__ __forceinline__ uint32_t to_words(const float* v, uint32_t* w) {
         for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
         return 0;
     }
-    uint32_t top = 0;
+    uint32_t top[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    const uint32_t s = mx::scale_code(top);
-    const float inv = mx::inverse_scale(s == 255u ? 0u : s);
+    for (int i = 0; i < 32; ++i) top[i & 3] = max(top[i & 3], __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    const uint32_t s = mx::scale_code(max(max(top[0], top[1]), max(top[2], top[3])));
+    const mx::f2 inv = mx::both(mx::inverse_scale(s == 255u ? 0u : s));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float q[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) q[k] = v[8 * i + k] * inv;
+        for (int k = 0; k < 4; ++k) mx::unpack2(mx::mul2(p[4 * i + k], inv), q[2 * k], q[2 * k + 1]);
         w[i] = s == 255u ? 0u : mx::pack_e2m1(q);
     }
     return s;
+}
+
+// adds the bias of 32 columns from `col` on; `whole`: all of them exist
+__device__ __forceinline__ void add_bias(mx::f2* v, const float* bias, int col, bool whole, int N) {
+    if (whole && ((uintptr_t)bias & 15u) == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 b = __ldg(reinterpret_cast<const float4*>(bias + col) + i);
+            v[2 * i] = mx::add2(v[2 * i], mx::pack2(b.x, b.y));
+            v[2 * i + 1] = mx::add2(v[2 * i + 1], mx::pack2(b.z, b.w));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            v[i] = mx::add2(v[i], mx::pack2(col + 2 * i < N ? __ldg(bias + col + 2 * i) : 0.0f, col + 2 * i + 1 < N ? __ldg(bias + col + 2 * i + 1) : 0.0f));
+    }
 }
 
 template <int OUT> struct Words { static constexpr int value = OUT == mx::KIND_BF16 ? 16 : OUT == mx::KIND_F32 ? 32 : 4; };
@@ -297,6 +316,7 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         constexpr int WORDS = Words<OUT>::value;
         constexpr int PER_BOX = OUT == mx::KIND_F32 ? 1 : 2;   // pieces per TMA store: 128 bytes of bf16 or f32, 32 of MXFP4
         uint8_t* patch = patches + (warp - 2) * PATCH_BYTES;
+        uint32_t scales = 0;
         int it = 0;
         bool ok = true;
         for (int tile = pair; tile < num_tiles; tile += num_pairs, ++it) {
@@ -329,39 +349,35 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 }
                 const int col = n0 + c;
                 if (row0 >= g.M) continue;
-                float v[32];
+                mx::f2 v[16];
                 const bool whole = col + 32 <= g.N;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(a[i]);
-                if (g.bias[0]) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] += whole || col + i < g.N ? __ldg(g.bias[0] + col + i) : 0.0f;
-                }
+                for (int i = 0; i < 16; ++i) v[i] = mx::pack2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
+                if (g.bias[0]) add_bias(v, g.bias[0], col, whole, g.N);
                 if (GATED) {
-                    float w[32];
+                    mx::f2 o[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(u[i]);
-                    if (g.bias[1]) {
+                    for (int i = 0; i < 16; ++i) o[i] = mx::pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+                    if (g.bias[1]) add_bias(o, g.bias[1], col, whole, g.N);
+                    mx::activate_pairs<16>(v, g.act);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] += whole || col + i < g.N ? __ldg(g.bias[1] + col + i) : 0.0f;
-                    }
-                    mx::activate32(v, g.act);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] *= w[i];
+                    for (int i = 0; i < 16; ++i) v[i] = mx::mul2(v[i], o[i]);
                 } else if (g.act == mx::ACT_RELU) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+                    mx::activate_pairs<16>(v, mx::ACT_RELU);
                 }
                 if (OUT == mx::KIND_MX && !whole) {            // (the same for a block wholly beyond the row's end: scale 0)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) if (col + i >= g.N) v[i] = 0.0f;
+                    for (int i = 0; i < 16; ++i) {
+                        if (col + 2 * i >= g.N) v[i] = 0;
+                        else if (col + 2 * i + 1 >= g.N) v[i] &= 0xFFFFFFFFull;
+                    }
                 }
                 uint32_t w[WORDS];
                 const uint32_t scale = to_words<OUT>(v, w);
-                if (OUT == mx::KIND_MX && row < g.M && (col >> 5) < (int)g.y_across * mx::TILE_BLOCKS)
-                    g.ys[mx::scale_offset(row, col >> 5, g.y_across)] = (uint8_t)scale;
                 const int col0 = n0 + (c & ~(32 * PER_BOX - 1));
                 if (!g.tma_store || col0 + 32 * PER_BOX > g.N) {
+                    if (OUT == mx::KIND_MX && row < g.M && (col >> 5) < (int)g.y_across * mx::TILE_BLOCKS)
+                        g.ys[mx::scale_offset(row, col >> 5, g.y_across)] = (uint8_t)scale;
                     if (row < g.M && col < g.N) store_direct<OUT>(g, row, col, w);
                     continue;
                 }
@@ -372,6 +388,11 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 }
                 if (OUT == mx::KIND_MX) {
                     *reinterpret_cast<uint4*>(patch + lane * 32 + half * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    scales |= scale << (8 * half);
+                    if (j % 2 == 1) {                                           // two neighbouring scales of the row
+                        if (row < g.M) *reinterpret_cast<uint16_t*>(g.ys + mx::scale_offset(row, col0 >> 5, g.y_across)) = (uint16_t)scales;
+                        scales = 0;
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < WORDS / 4; ++i)                         // 128-byte swizzle: 16-byte piece p of row r at p ^ (r & 7)

@@ -215,29 +215,79 @@ inline bool make_out_map(CUtensorMap* map, void* base, int kind, long long rows,
 // ---- activations of the gated Dense -------------------------------------------------------------
 constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_SIGMOID = 5, ACT_COUNT = 6;
 
-// 1 / (1 + exp(-x)) in float32: exp overflows to infinity for x below -88 and the quotient is then 0, as it should be
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
-
-__device__ __forceinline__ float activate(float x, int act) {
-    switch (act) {
-        case ACT_RELU: return x < 0.0f ? 0.0f : x;      // a NaN stays one
-        case ACT_SILU: return x * sigmoid(x);
-        case ACT_GELU: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-        // 0.5 (1 + tanh z) = sigmoid(2 z)
-        case ACT_GELU_TANH: return x * sigmoid(1.5957691216057308f * (x + 0.044715f * x * x * x));
-        case ACT_SIGMOID: return sigmoid(x);
-        default: return x;
-    }
+// Two float32 values in a 64-bit register pair: one instruction for both, half the issue slots of an epilogue.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float lo, float hi) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ f2 both(float x) { return pack2(x, x); }
+__device__ __forceinline__ void unpack2(f2 p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float rcp_approx(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+template <float (*F)(float)>
+__device__ __forceinline__ f2 each2(f2 p) {
+    float a, b;
+    unpack2(p, a, b);
+    return pack2(F(a), F(b));
 }
 
-// the switch outside the loop: 32 values of one activation
-__device__ __forceinline__ void activate32(float* v, int act) {
+constexpr float LOG2E = 1.4426950408889634f;
+
+// 1 / (1 + 2^z): 2^z overflows to infinity where the quotient is 0, as it should be
+__device__ __forceinline__ f2 inv_one_plus_exp2(f2 z) { return each2<rcp_approx>(add2(each2<exp2_approx>(z), both(1.0f))); }
+
+// x Phi(x) = max(x, 0) - |x| / 2 erfc(|x| / sqrt 2), erfc by formula 7.1.26 of Abramowitz and Stegun (Handbook of
+// Mathematical Functions): t (a1 + t (a2 + ...)) exp(-z^2), t = 1 / (1 + p z), absolute error at most 1.5e-7.  erff would
+// take twice the instructions, and 1 + erf cancels for negative x.
+__device__ __forceinline__ f2 gelu2(f2 x) {
+    const f2 ax = x & 0x7FFFFFFF7FFFFFFFull;
+    const f2 t = each2<rcp_approx>(fma2(ax, both(0.3275911f * 0.70710678118654752f), both(1.0f)));
+    f2 p = fma2(t, both(1.061405429f), both(-1.453152027f));
+    p = fma2(t, p, both(1.421413741f));
+    p = fma2(t, p, both(-0.284496736f));
+    p = fma2(t, p, both(0.254829592f));
+    const f2 e = each2<exp2_approx>(mul2(mul2(x, both(-0.5f * LOG2E)), x));
+    const f2 h = mul2(mul2(ax, both(-0.5f)), mul2(t, p));
+    float a, b;
+    unpack2(x, a, b);
+    return fma2(h, e, pack2(a < 0.0f ? 0.0f : a, b < 0.0f ? 0.0f : b));     // a NaN stays one
+}
+
+template <int ACT>
+__device__ __forceinline__ f2 activate2(f2 x) {
+    if (ACT == ACT_RELU) {
+        float a, b;
+        unpack2(x, a, b);
+        return pack2(a < 0.0f ? 0.0f : a, b < 0.0f ? 0.0f : b);
+    }
+    if (ACT == ACT_SILU) return mul2(x, inv_one_plus_exp2(mul2(x, both(-LOG2E))));
+    if (ACT == ACT_SIGMOID) return inv_one_plus_exp2(mul2(x, both(-LOG2E)));
+    if (ACT == ACT_GELU) return gelu2(x);
+    if (ACT == ACT_GELU_TANH) {      // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z)), z = sqrt(2 / pi) (x + 0.044715 x^3)
+        constexpr float C = -2.0f * 0.79788456080286536f * LOG2E;
+        const f2 z = mul2(x, fma2(mul2(x, x), both(0.044715f * C), both(C)));
+        return mul2(x, inv_one_plus_exp2(z));
+    }
+    return x;
+}
+
+// N pairs of one activation, the switch outside the loop
+template <int N>
+__device__ __forceinline__ void activate_pairs(f2* v, int act) {
     switch (act) {
-#define A4C_MX_EACH(A) case A: _Pragma("unroll") for (int i = 0; i < 32; ++i) v[i] = activate(v[i], A); break;
+#define A4C_MX_EACH(A) case A: _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = activate2<A>(v[i]); break;
         A4C_MX_EACH(ACT_RELU) A4C_MX_EACH(ACT_SILU) A4C_MX_EACH(ACT_GELU) A4C_MX_EACH(ACT_GELU_TANH) A4C_MX_EACH(ACT_SIGMOID)
 #undef A4C_MX_EACH
         default: break;
     }
+}
+__device__ __forceinline__ float activate(float x, int act) {
+    f2 v = both(x);
+    activate_pairs<1>(&v, act);
+    float a, b;
+    unpack2(v, a, b);
+    return a;
 }
 
 }  // namespace mx
