@@ -17,8 +17,8 @@
 // by the MMA thread they run in turn with the MMAs, six copies of a stage costing 0.22 us on top of its 0.40 us of MMAs
 // (4096 x 16384 x 8192: 303 us; spread out between the MMAs 346 us; from their own warp 240 us, no copies at all 205 us).
 //
-// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-9 epilogue in two groups of four, each half of the columns, 10 scale
-// copies (leader CTA).  A lane holds one row, so an MXFP4 output block is 32 registers of one thread; rows go out through a
+// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2 scale copies (leader CTA), 3-10
+// epilogue in two groups of four, each half of the columns.  A lane holds one row, so an MXFP4 output block is 32 registers of one thread; rows go out through a
 // swizzled patch of shared memory per warp and TMA stores (directly from registers every 16 bytes of a row were an L2
 // request of their own).  Every wait is bounded.
 #include <cuda.h>
@@ -45,7 +45,8 @@ constexpr int SF0 = TMEM_COLS - SF_SETS * SF_COLS;
 constexpr int ACC1 = SF0 - BN;                // second accumulator: columns ACC1 .. SF0
 constexpr int OVERLAP = BN - ACC1;
 constexpr int EPI_WARPS = 8;
-constexpr int NUM_THREADS = 96 + EPI_WARPS * 32;
+constexpr int EPI_WARP0 = 3;                   // first epilogue warp
+constexpr int NUM_THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
 constexpr int PATCH_BYTES = 32 * 128;           // per epilogue warp: 32 rows of a TMA store's box
 
 struct Tail {
@@ -115,22 +116,6 @@ __device__ __forceinline__ uint32_t to_words(const mx::f2* p, uint32_t* w) {
     return s;
 }
 
-// adds the bias of 32 columns from `col` on; `whole`: all of them exist
-__device__ __forceinline__ void add_bias(mx::f2* v, const float* bias, int col, bool whole, int N) {
-    if (whole && ((uintptr_t)bias & 15u) == 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 b = __ldg(reinterpret_cast<const float4*>(bias + col) + i);
-            v[2 * i] = mx::add2(v[2 * i], mx::pack2(b.x, b.y));
-            v[2 * i + 1] = mx::add2(v[2 * i + 1], mx::pack2(b.z, b.w));
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            v[i] = mx::add2(v[i], mx::pack2(col + 2 * i < N ? __ldg(bias + col + 2 * i) : 0.0f, col + 2 * i + 1 < N ? __ldg(bias + col + 2 * i + 1) : 0.0f));
-    }
-}
-
 template <int OUT> struct Words { static constexpr int value = OUT == mx::KIND_BF16 ? 16 : OUT == mx::KIND_F32 ? 32 : 4; };
 
 // straight from registers: for outputs that a tensor map cannot describe, and for boxes that reach beyond the row's end (a TMA
@@ -163,6 +148,66 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+// adds the bias of 32 neighbouring columns from `col` on; columns beyond the row's end get none
+__device__ __forceinline__ void add_bias(mx::f2* v, const float* bias, int col, int cols) {
+    if (col + 32 <= cols && ((uintptr_t)bias & 15u) == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 b = __ldg(reinterpret_cast<const float4*>(bias + col) + i);
+            v[2 * i] = mx::add2(v[2 * i], mx::pack2(b.x, b.y));
+            v[2 * i + 1] = mx::add2(v[2 * i + 1], mx::pack2(b.z, b.w));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            v[i] = mx::add2(v[i], mx::pack2(col + 2 * i < cols ? __ldg(bias + col + 2 * i) : 0.0f, col + 2 * i + 1 < cols ? __ldg(bias + col + 2 * i + 1) : 0.0f));
+    }
+}
+
+// 32 finished neighbouring values of each lane's row, `half` 0 or 1 of 64 (called for both, `first` says which comes first)
+// -> output and, for MXFP4, the two scales of the 64; a block that lies beyond the row's end gets scale 0
+template <int OUT>
+__device__ __forceinline__ void store32(const Args& g, const CUtensorMap* map_y, uint8_t* patch, long long row0, int lane, int col, int half,
+                                        bool first, uint32_t& scales, mx::f2* v) {
+    const long long row = row0 + lane;
+    constexpr int WORDS = Words<OUT>::value;
+    constexpr int BOX = OUT == mx::KIND_F32 ? 32 : 64;     // columns per TMA store: 128 bytes of bf16 or f32, 32 of MXFP4
+    const int col64 = col - 32 * half;
+    const bool boxed = g.tma_store && (BOX == 32 ? col : col64) + BOX <= g.N;
+    if (OUT == mx::KIND_MX && col + 32 > g.N) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (col + 2 * i >= g.N) v[i] = 0;
+            else if (col + 2 * i + 1 >= g.N) v[i] &= 0xFFFFFFFFull;
+        }
+    }
+    uint32_t w[WORDS];
+    scales = (first ? 0u : scales) | to_words<OUT>(v, w) << (8 * half);
+    if (OUT == mx::KIND_MX && !first && row < g.M && (col64 >> 5) < (int)g.y_across * mx::TILE_BLOCKS)
+        *reinterpret_cast<uint16_t*>(g.ys + mx::scale_offset(row, col64 >> 5, g.y_across)) = (uint16_t)scales;
+    if (!boxed) {
+        if (row < g.M && col < g.N) store_direct<OUT>(g, row, col, w);
+        return;
+    }
+    if (BOX == 32 || first) {                              // the patch's last store has been read
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+    }
+    if (OUT == mx::KIND_MX) {
+        *reinterpret_cast<uint4*>(patch + lane * 32 + half * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; ++i)                // 128-byte swizzle: 16-byte piece p of row r at p ^ (r & 7)
+            *reinterpret_cast<uint4*>(patch + lane * 128 + ((((BOX == 64 ? half * 4 : 0) + i) ^ (lane & 7)) << 4)) =
+                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+    if (BOX == 32 || !first) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tma_store_2d(map_y, patch, OUT == mx::KIND_MX ? col64 / 2 : BOX == 32 ? col : col64, (int)row0);
+    }
+}
 
 template <bool GATED, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
@@ -274,7 +319,7 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             }
         }
         __syncwarp();
-    } else if (warp == 10) {
+    } else if (warp == 2) {
         if (leader && lane == 0) {
             const int total = ((num_tiles - pair + num_pairs - 1) / num_pairs) * g.num_kb;
             int stage = 0, kb = 0;
@@ -305,107 +350,89 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         __syncwarp();
     } else {
         const int quad = warp & 3;
-        const int grp = (warp - 2) >> 2;
+        const int grp = (warp - EPI_WARP0) >> 2;
         const uint32_t lane_base = tmem_base + ((uint32_t)(quad * 32) << 16);
-        constexpr int CHUNKS = GATED ? 2 : 4;                  // pieces of 32 output columns per group
-        constexpr int GROUP_COLS = CHUNKS * 32;
-        // pieces until the overlapping columns are in registers (they are the last of accumulator 0, the first of 1; for the
-        // gated Dense the second factor's last columns and the gate's first ones)
-        constexpr int OVERLAP_CHUNKS = (OVERLAP + 31) / 32;
-        static_assert(OVERLAP_CHUNKS <= CHUNKS, "the overlap lies within one group's columns");
-        constexpr int WORDS = Words<OUT>::value;
-        constexpr int PER_BOX = OUT == mx::KIND_F32 ? 1 : 2;   // pieces per TMA store: 128 bytes of bf16 or f32, 32 of MXFP4
-        uint8_t* patch = patches + (warp - 2) * PATCH_BYTES;
+        constexpr int HALF = 64;                               // columns per TMEM load step; the overlap lies within one
+        static_assert(OVERLAP <= HALF, "the overlap lies within one load step");
+        constexpr int COLS = GATED ? 64 : 128;                 // output columns per group
+        uint8_t* patch = patches + (warp - EPI_WARP0) * PATCH_BYTES;
         uint32_t scales = 0;
         int it = 0;
         bool ok = true;
+        auto release = [&](uint64_t* bar) {                    // this warp's part of an accumulator is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mx::mbar_arrive_cluster(mx::map_to_cta(smem_u32(bar), 0));
+        };
+        // Dense: all of a thread's 128 accumulator values go to registers before any is converted, the columns that the two
+        // accumulators share first, so the next tile's MMAs wait for the loads only and never for the arithmetic.
+        auto dense_tile = [&](int acc, long long row0, int n0) {
+            const uint32_t taddr = lane_base + (uint32_t)((acc ? ACC1 : 0) + grp * COLS);
+            const int up = acc ? 0 : 1;                        // the load step, and the group, that holds the shared columns
+            uint32_t r[4][32];                                 // pieces of 32 columns: of the first load step, then of the other
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t at = taddr + (uint32_t)((i ^ up) * HALF);
+                tmem_ld32_async(at, r[2 * i]);
+                tmem_ld32_async(at + 32u, r[2 * i + 1]);
+                tmem_ld_wait32(r[2 * i]);
+                tmem_ld_wait32(r[2 * i + 1]);
+                if (i == 0 && grp == up) release(&tail->overlap_free[acc]);
+                if (i == 1) release(&tail->tmem_empty[acc]);
+            }
+            if (row0 >= g.M) return;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const int col = n0 + grp * COLS + ((p >> 1) ^ up) * HALF + 32 * (p & 1);
+                mx::f2 v[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = mx::pack2(__uint_as_float(r[p][2 * k]), __uint_as_float(r[p][2 * k + 1]));
+                if (g.bias[0]) add_bias(v, g.bias[0], col, g.N);
+                if (g.act == mx::ACT_RELU) mx::activate_pairs<16>(v, mx::ACT_RELU);
+                store32<OUT>(g, &map_y, patch, row0, lane, col, p & 1, (p & 1) == 0, scales, v);
+            }
+        };
+        // Gated: 32 outputs at a time (64 registers of accumulators beside the activation's own); all at once as above spilled and
+        // ran 15 % slower on short reductions.  The shared columns are the second factor's last (accumulator 0) or the gate's
+        // first, so those pieces come first.
+        auto gated_tile = [&](int acc, long long row0, int n0) {
+            const uint32_t taddr = lane_base + (uint32_t)((acc ? ACC1 : 0) + grp * COLS);
+            const int up = acc == 0 && grp == 1;
+#pragma unroll 1
+            for (int j = 0; j < 2; ++j) {
+                const int half = j ^ up;
+                uint32_t a[32], u[32];
+                tmem_ld32_async(taddr + (uint32_t)(32 * half), a);
+                tmem_ld32_async(taddr + (uint32_t)(128 + 32 * half), u);
+                tmem_ld_wait32(a);
+                tmem_ld_wait32(u);
+                if (j == 1 && grp == 1 - acc) release(&tail->overlap_free[acc]);
+                if (j == 1) release(&tail->tmem_empty[acc]);
+                if (row0 >= g.M) continue;
+                const int col = n0 + grp * COLS + 32 * half;
+                mx::f2 v[16], w[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    v[k] = mx::pack2(__uint_as_float(a[2 * k]), __uint_as_float(a[2 * k + 1]));
+                    w[k] = mx::pack2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
+                }
+                if (g.bias[0]) add_bias(v, g.bias[0], col, g.N);
+                if (g.bias[1]) add_bias(w, g.bias[1], col, g.N);
+                mx::activate_pairs<16>(v, g.act);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = mx::mul2(v[k], w[k]);
+                store32<OUT>(g, &map_y, patch, row0, lane, col, half, j == 0, scales, v);
+            }
+        };
         for (int tile = pair; tile < num_tiles; tile += num_pairs, ++it) {
             int mt, nt;
             tile_coords(tile, g, mt, nt);
-            const int acc = it & 1;
-            const long long row0 = (long long)mt * BM + (int)rank * BM_CTA + quad * 32, row = row0 + lane;
-            const int n0 = nt * OUT_COLS;
-            if (ok) ok = mbar_wait(&tail->tmem_full[acc], (it >> 1) & 1, abort_flag, g.status, 165);
+            const long long row0 = (long long)mt * BM + (int)rank * BM_CTA + quad * 32;
+            if (ok) ok = mbar_wait(&tail->tmem_full[it & 1], (it >> 1) & 1, abort_flag, g.status, 165);
             if (!ok) continue;
             tc_fence_after();
-            const uint32_t taddr = lane_base + (uint32_t)(acc ? ACC1 : 0);
-            const bool holds_overlap = acc ? grp == 0 : grp == 1;
-            const bool down = acc == 0 && grp == 1;            // from the top, where accumulator 0 overlaps
-#pragma unroll 1
-            for (int j = 0; j < CHUNKS; ++j) {
-                const int c = grp * GROUP_COLS + 32 * (down ? CHUNKS - 1 - j : j);
-                uint32_t a[32], u[32];
-                tmem_ld32_async(taddr + (uint32_t)c, a);
-                if (GATED) { tmem_ld32_async(taddr + (uint32_t)(128 + c), u); tmem_ld_wait32(u); }
-                tmem_ld_wait32(a);
-                const bool last = j == CHUNKS - 1, over = holds_overlap && j == OVERLAP_CHUNKS - 1;
-                if (last || over) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (over) mx::mbar_arrive_cluster(mx::map_to_cta(smem_u32(&tail->overlap_free[acc]), 0));
-                        if (last) mx::mbar_arrive_cluster(mx::map_to_cta(smem_u32(&tail->tmem_empty[acc]), 0));
-                    }
-                }
-                const int col = n0 + c;
-                if (row0 >= g.M) continue;
-                mx::f2 v[16];
-                const bool whole = col + 32 <= g.N;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = mx::pack2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
-                if (g.bias[0]) add_bias(v, g.bias[0], col, whole, g.N);
-                if (GATED) {
-                    mx::f2 o[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = mx::pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-                    if (g.bias[1]) add_bias(o, g.bias[1], col, whole, g.N);
-                    mx::activate_pairs<16>(v, g.act);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = mx::mul2(v[i], o[i]);
-                } else if (g.act == mx::ACT_RELU) {
-                    mx::activate_pairs<16>(v, mx::ACT_RELU);
-                }
-                if (OUT == mx::KIND_MX && !whole) {            // (the same for a block wholly beyond the row's end: scale 0)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (col + 2 * i >= g.N) v[i] = 0;
-                        else if (col + 2 * i + 1 >= g.N) v[i] &= 0xFFFFFFFFull;
-                    }
-                }
-                uint32_t w[WORDS];
-                const uint32_t scale = to_words<OUT>(v, w);
-                const int col0 = n0 + (c & ~(32 * PER_BOX - 1));
-                if (!g.tma_store || col0 + 32 * PER_BOX > g.N) {
-                    if (OUT == mx::KIND_MX && row < g.M && (col >> 5) < (int)g.y_across * mx::TILE_BLOCKS)
-                        g.ys[mx::scale_offset(row, col >> 5, g.y_across)] = (uint8_t)scale;
-                    if (row < g.M && col < g.N) store_direct<OUT>(g, row, col, w);
-                    continue;
-                }
-                const int half = PER_BOX == 2 ? (c >> 5) & 1 : 0;              // which half of the box's columns
-                if (j % PER_BOX == 0) {                                         // the patch's last store has been read
-                    if (lane == 0) tma_store_wait_read();
-                    __syncwarp();
-                }
-                if (OUT == mx::KIND_MX) {
-                    *reinterpret_cast<uint4*>(patch + lane * 32 + half * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-                    scales |= scale << (8 * half);
-                    if (j % 2 == 1) {                                           // two neighbouring scales of the row
-                        if (row < g.M) *reinterpret_cast<uint16_t*>(g.ys + mx::scale_offset(row, col0 >> 5, g.y_across)) = (uint16_t)scales;
-                        scales = 0;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < WORDS / 4; ++i)                         // 128-byte swizzle: 16-byte piece p of row r at p ^ (r & 7)
-                        *reinterpret_cast<uint4*>(patch + lane * 128 + (((half * 4 + i) ^ (lane & 7)) << 4)) =
-                            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                }
-                if (j % PER_BOX == PER_BOX - 1) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0)
-                        tma_store_2d(&map_y, patch, OUT == mx::KIND_MX ? col0 / 2 : col0, (int)row0);
-                }
-            }
+            if (GATED) gated_tile(it & 1, row0, nt * OUT_COLS);
+            else dense_tile(it & 1, row0, nt * OUT_COLS);
         }
         if (lane == 0) tma_store_wait_read();      // the patch outlives its last store
     }
