@@ -9,9 +9,10 @@
 //
 // With few rows the time is the weights' way out of memory, so the weights are the M operand here (128 of them to a
 // tile) and the rows of A the N operand (16 to 128): a tile fetches 16 KB of weights for 2 KB of A at 16 rows, where the
-// other way round every tile would carry 128 mostly empty rows.  When there are fewer tiles than SMs the reduction is
-// split over a cluster of up to 8 CTAs: each leaves its partial tile in its own shared memory and the ranks add them up
-// in rank order over distributed shared memory, so the result does not depend on timing and no workspace exists.
+// other way round every tile would carry 128 mostly empty rows.  While that leaves SMs idle the row tiles get smaller, down
+// to 32 (the weights' second fetch comes from the L2), and then the reduction is split over a cluster of up to 8 CTAs: each
+// rank sends its partial sums to the rank that finishes the row (distributed shared memory), which adds them in rank order,
+// so the result does not depend on timing and no workspace exists.
 //
 // One tile per CTA: warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue.  A stage is 256 values of K: 128-byte
 // swizzled rows of codes and the scale tiles, which tcgen05.cp moves on to TMEM ahead of the stage's MMAs (the tensor
@@ -34,12 +35,14 @@ constexpr int SF_BYTES = 2 * mx::TILE_BYTES;  // scales of 128 rows x 256 values
 constexpr int NUM_THREADS = 192;
 constexpr int MAX_STAGES = 12;
 constexpr int MAX_SPLIT = 8;                  // portable cluster size
+constexpr int SPLIT_T = 32;                   // most rows per tile when the reduction is split
 constexpr int SMEM_BUDGET = 200 * 1024;
 constexpr size_t ONE_PER_SM = 116 * 1024;
 
 struct Tail {
     uint64_t full[MAX_STAGES];
     uint64_t empty[MAX_STAGES];
+    uint64_t moved[MAX_STAGES];      // the stage's A scales lie in the first column
     uint64_t done;
     uint32_t tmem_base;
     volatile int abort_flag;
@@ -55,19 +58,18 @@ struct Args {
     int N, K;
     int k_tiles;                     // scale tiles across K
     int num_kb;                      // stages of the whole reduction
-    int t;                           // rows of A per tile (multiple of 16)
+    int t;                           // rows of A per tile: 16, 32, 64 or 128
     int split;                       // CTAs per tile (cluster size)
     int num_n_tiles;
-    int stages, stage_bytes;
+    int stages, stage_bytes;         // the partial sums of a split reduction lie behind the stages
+    int part_bytes;
     int out_kind, act;
     uint32_t idesc;
     int* status;
 };
 
-__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mx::map_to_cta(local, rank)) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster(uint32_t local, uint32_t rank, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(mx::map_to_cta(local, rank)), "f"(v) : "memory");
 }
 
 // One value of row m and feature n (this lane's), complete over K; the 32 lanes of a warp hold 32 neighbouring
@@ -120,56 +122,68 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     constexpr int TMEM_COLS = GATED ? 512 : 256;      // a power of two >= SF0 + 2 * SF_COLS
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    Tail* tail = reinterpret_cast<Tail*>(smem + (size_t)g.stages * g.stage_bytes);
+    float* part = reinterpret_cast<float*>(smem + (size_t)g.stages * g.stage_bytes);
+    Tail* tail = reinterpret_cast<Tail*>(smem + (size_t)g.stages * g.stage_bytes + g.part_bytes);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t rank = mx::cluster_rank();
     const int tile = (int)(blockIdx.x / (unsigned)g.split);
-    const long long m0 = (long long)(tile / g.num_n_tiles) * MAX_T;   // t < MAX_T only when there is one row tile
+    const long long m0 = (long long)(tile / g.num_n_tiles) * g.t;
     const int n0 = (tile % g.num_n_tiles) * BN;
     const int kb0 = (int)((long long)g.num_kb * rank / g.split), kb1 = (int)((long long)g.num_kb * (rank + 1) / g.split);
 
+    // A column of TMEM holds 32 rows' scales, and an MMA reads them from a multiple of 4 columns on.  A row tile that does not
+    // begin with a scale tile has its scales moved to the first column while they are in shared memory.
+    const int sf_row = (int)(m0 % mx::TILE_ROWS) / 32;
+    volatile int* abort_flag = &tail->abort_flag;
+    const int a_bytes = g.t * (BK / 2);
+
+    // stage: W (and Wu) codes, A codes, then the scales of W (and Wu) and of A
+    auto load = [&](int kb, int stage) {
+        uint8_t* s = smem + (size_t)stage * g.stage_bytes;
+        uint64_t* bar = &tail->full[stage];
+        const uint32_t sf = (uint32_t)min(2, g.k_tiles - 2 * kb) * mx::TILE_BYTES;
+        const long long w_off = ((long long)(n0 / mx::TILE_ROWS) * g.k_tiles + 2 * kb) * mx::TILE_BYTES;
+        mbar_arrive_expect_tx(bar, (uint32_t)(NW * W_BYTES + a_bytes) + (NW + 1) * sf);
+        tma_load_2d(s, &map_w, bar, kb * (BK / 2), n0);
+        if (GATED) tma_load_2d(s + W_BYTES, &map_u, bar, kb * (BK / 2), n0);
+        tma_load_2d(s + NW * W_BYTES, &map_a, bar, kb * (BK / 2), (int)m0);
+        uint8_t* f = s + g.stage_bytes - (NW + 1) * SF_BYTES;
+        mx::bulk_load(f, g.sw[0] + w_off, sf, bar);
+        if (GATED) mx::bulk_load(f + SF_BYTES, g.sw[1] + w_off, sf, bar);
+        mx::bulk_load(f + NW * SF_BYTES, g.sa + ((m0 / mx::TILE_ROWS) * g.k_tiles + 2 * kb) * mx::TILE_BYTES, sf, bar);
+    };
+    const int ahead = min(g.stages, kb1 - kb0);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < g.stages; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); }
+        for (int s = 0; s < g.stages; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); mbar_init(&tail->moved[s], 1); }
         mbar_init(&tail->done, 1);
         tail->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        mx::grid_wait();
+        for (int i = 0; i < ahead; ++i) load(kb0 + i, i);      // the first round needs no slot to be emptied
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      :: "r"(smem_u32(&tail->tmem_base)), "r"((uint32_t)TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    mx::grid_wait();
+    mx::grid_release();
+    if (g.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this rank's memory may be written
     const uint32_t tmem_base = tail->tmem_base;
-    volatile int* abort_flag = &tail->abort_flag;
-    const int a_bytes = g.t * (BK / 2);
 
-    // stage: W (and Wu) codes, A codes, then the scales of W (and Wu) and of A
     if (warp == 0) {
         if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
-            const uint8_t* sf_w = g.sw[0] + (long long)(n0 / mx::TILE_ROWS) * g.k_tiles * mx::TILE_BYTES;
-            const uint8_t* sf_u = GATED ? g.sw[1] + (long long)(n0 / mx::TILE_ROWS) * g.k_tiles * mx::TILE_BYTES : nullptr;
-            const uint8_t* sf_a = g.sa + (m0 / mx::TILE_ROWS) * g.k_tiles * mx::TILE_BYTES;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(&tail->empty[stage], phase ^ 1u, abort_flag, g.status, 151)) break;
-                uint8_t* s = smem + (size_t)stage * g.stage_bytes;
-                uint64_t* bar = &tail->full[stage];
-                const uint32_t sf = (uint32_t)min(2, g.k_tiles - 2 * kb) * mx::TILE_BYTES;
-                const long long sf_off = (long long)kb * SF_BYTES;
-                mbar_arrive_expect_tx(bar, (uint32_t)(NW * W_BYTES + a_bytes) + (NW + 1) * sf);
-                tma_load_2d(s, &map_w, bar, kb * (BK / 2), n0);
-                if (GATED) tma_load_2d(s + W_BYTES, &map_u, bar, kb * (BK / 2), n0);
-                tma_load_2d(s + NW * W_BYTES, &map_a, bar, kb * (BK / 2), (int)m0);
-                uint8_t* f = s + g.stage_bytes - (NW + 1) * SF_BYTES;
-                mx::bulk_load(f, sf_w + sf_off, sf, bar);
-                if (GATED) mx::bulk_load(f + SF_BYTES, sf_u + sf_off, sf, bar);
-                mx::bulk_load(f + NW * SF_BYTES, sf_a + sf_off, sf, bar);
+            for (int kb = kb0 + ahead; kb < kb1; ++kb) {
+                if (!mbar_wait(&tail->empty[stage], phase, abort_flag, g.status, 151)) break;
+                load(kb, stage);
                 if (++stage == g.stages) { stage = 0; phase ^= 1u; }
             }
         }
@@ -180,7 +194,8 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             uint32_t phase = 0;
             bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb) {
-                ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 152);
+                ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 152) &&
+                     (sf_row == 0 || mbar_wait(&tail->moved[stage], phase, abort_flag, g.status, 154));
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t s = smem_u32(smem) + (uint32_t)(stage * g.stage_bytes);
@@ -209,6 +224,21 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (++stage == g.stages) { stage = 0; phase ^= 1u; }
             }
             if (ok) umma_commit(&tail->done);
+        }
+        __syncwarp();
+    } else if (warp == 2 && sf_row != 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 155)) break;
+            uint32_t* f = reinterpret_cast<uint32_t*>(smem + (size_t)(stage + 1) * g.stage_bytes - SF_BYTES) + lane * 4;
+            const bool two = g.k_tiles - 2 * kb > 1;
+            f[0] = f[sf_row];
+            if (two) f[mx::TILE_BYTES / 4] = f[mx::TILE_BYTES / 4 + sf_row];
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tail->moved[stage]);
+            if (++stage == g.stages) { stage = 0; phase ^= 1u; }
         }
         __syncwarp();
     }
@@ -243,9 +273,11 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
         }
     } else {
-        // the partial tile [row][feature] in the stage buffers: all loads and MMAs of this CTA are complete
-        float* part = reinterpret_cast<float*>(smem);
+        // row r is finished by rank r mod split; part[from][r / split][projection][feature] there
+        const int per = g.t / g.split;
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // every rank has started
         if (ok) {
+            const uint32_t base = smem_u32(part) + (uint32_t)((int)rank * per * NW * BN + nl) * 4u;
 #pragma unroll 1
             for (int c = 0; c < rows; c += 16)
 #pragma unroll
@@ -258,23 +290,28 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         : "r"(taddr + (uint32_t)(o * MAX_T + c)));
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) part[(o * g.t + c + i) * BN + nl] = __uint_as_float(a[i]);
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = c + i;
+                        if (r < rows)
+                            st_cluster(base + (uint32_t)((r / g.split) * NW + o) * (BN * 4u), (uint32_t)(r & (g.split - 1)), __uint_as_float(a[i]));
+                    }
                 }
         }
-        __syncthreads();
-        mx::cluster_sync_all();
+        __syncwarp();
+        mx::cluster_sync_all();          // all partial sums have arrived
         if (warp >= 2) {
-            const uint32_t base = smem_u32(part) + (uint32_t)(nl * 4);
             for (int r = (int)rank; r < rows; r += g.split) {
+                const float* p = part + (r / g.split) * NW * BN + nl;
                 float a = 0.0f, u = 0.0f;
-                for (int q = 0; q < g.split; ++q) {
-                    a += ld_cluster(base + (uint32_t)(r * BN * 4), (uint32_t)q);
-                    if (GATED) u += ld_cluster(base + (uint32_t)((g.t + r) * BN * 4), (uint32_t)q);
-                }
+#pragma unroll
+                for (int q = 0; q < MAX_SPLIT; ++q)
+                    if (q < g.split) {
+                        a += p[q * per * NW * BN];
+                        if (GATED) u += p[q * per * NW * BN + BN];
+                    }
                 if (ok) store_value(g, m0 + r, n, finish_value<GATED>(g, a, u, ba, bu));
             }
         }
-        mx::cluster_sync_all();      // nobody leaves while another rank reads its memory
     }
 
     tc_fence_before();
@@ -296,19 +333,7 @@ cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mw, const CUtensorM
     static tc::SmemOptIn opt_in;
     const cudaError_t e = opt_in.ensure(dense_mx_kernel<GATED>, SMEM_BUDGET + 16 * 1024);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(NUM_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)g.split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, dense_mx_kernel<GATED>, ma, mw, mu, g);
+    return mx::launch_serialized(dense_mx_kernel<GATED>, grid, NUM_THREADS, smem, (unsigned)g.split, s, ma, mw, mu, g);
 }
 
 }  // namespace
@@ -326,23 +351,24 @@ int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stre
     g.M = d.M; g.N = d.N; g.K = d.K; g.k_tiles = (int)mx::tiles_across(d.K);
     g.num_kb = (d.K + BK - 1) / BK;
     g.out_kind = d.out_kind; g.act = d.act; g.status = status_word;
-    g.t = d.M >= MAX_T ? MAX_T : (int)((d.M + 15) / 16 * 16);
     g.num_n_tiles = (d.N + BN - 1) / BN;
-    const long long tiles = (d.M + MAX_T - 1) / MAX_T * g.num_n_tiles;
-    if (tiles > 2147483647LL / MAX_SPLIT) return A4C_ERR_TOO_LARGE;
-    // split the reduction while a CTA per SM is not reached and every rank keeps a stage
+    g.t = d.M > 64 ? 128 : d.M > 32 ? 64 : d.M > 16 ? 32 : 16;
+    auto tiles_of = [&](int t) { return (d.M + t - 1) / t * g.num_n_tiles; };
+    if (tiles_of(g.t) > 2147483647LL / MAX_SPLIT) return A4C_ERR_TOO_LARGE;
+    // Smaller row tiles, then a split reduction, while at most half of the SMs have work and every rank keeps a stage.
+    while (g.t > SPLIT_T && tiles_of(g.t) * 2 <= sms) g.t /= 2;
+    const long long tiles = tiles_of(g.t);
     g.split = 1;
-    while (g.split < MAX_SPLIT && tiles * g.split * 2 <= sms && g.split * 2 <= g.num_kb) g.split *= 2;
+    while (g.split < MAX_SPLIT && g.t <= SPLIT_T && tiles * g.split * 2 <= sms && g.split * 2 <= g.num_kb) g.split *= 2;
     g.idesc = mx::make_idesc(BN, g.t);
     g.stage_bytes = nw * W_BYTES + g.t * (BK / 2) + (nw + 1) * SF_BYTES;
     const int need = (g.num_kb + g.split - 1) / g.split;
-    int stages = SMEM_BUDGET / g.stage_bytes;
+    int stages = (SMEM_BUDGET - (g.split > 1 ? nw * g.t * BN * 4 : 0)) / g.stage_bytes;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
-    const int part_bytes = g.split > 1 ? nw * g.t * BN * 4 : 0;       // the partial tile lies over the stages
-    int least = (part_bytes + g.stage_bytes - 1) / g.stage_bytes;
-    if (need < stages) stages = need > least ? need : least;
+    if (need < stages) stages = need;
     g.stages = stages;
-    size_t smem = 1024 + (size_t)g.stages * g.stage_bytes + sizeof(Tail);
+    g.part_bytes = g.split > 1 ? nw * g.t * BN * 4 : 0;
+    size_t smem = 1024 + (size_t)g.stages * g.stage_bytes + g.part_bytes + sizeof(Tail);
     // More than half of an SM's shared memory, so that one CTA lives on an SM at a time: the ranks of a cluster wait for
     // one another while they hold tensor memory, and two clusters that shared SMs could each wait for the other's.
     if (smem < ONE_PER_SM) smem = ONE_PER_SM;

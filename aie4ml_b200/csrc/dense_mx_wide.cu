@@ -248,6 +248,8 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     __syncthreads();
     mx::cluster_sync_all();
     tc_fence_after();
+    mx::grid_wait();
+    mx::grid_release();
     const uint32_t tmem_base = tail->tmem_base;
     volatile int* abort_flag = &tail->abort_flag;
 
@@ -455,8 +457,7 @@ cudaError_t launch(const CUtensorMap* m, const Args& g, int grid, cudaStream_t s
     static tc::SmemOptIn opt_in;
     const cudaError_t e = opt_in.ensure(dense_mx_wide_kernel<GATED, OUT>, SMEM_BYTES);
     if (e != cudaSuccess) return e;
-    dense_mx_wide_kernel<GATED, OUT><<<grid, NUM_THREADS, SMEM_BYTES, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], m[6], g);
-    return cudaGetLastError();
+    return mx::launch_serialized(dense_mx_wide_kernel<GATED, OUT>, (unsigned)grid, NUM_THREADS, SMEM_BYTES, 0, s, m[0], m[1], m[2], m[3], m[4], m[5], m[6], g);
 }
 
 }  // namespace

@@ -109,6 +109,33 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 
+// ---- back-to-back launches ----------------------------------------------------------------------
+// The MXFP4 kernels are launched with programmatic stream serialization: a kernel may be set up (barriers, tensor memory)
+// while the one before it in the stream drains.  Nothing in global memory is read or written ahead of grid_wait, which
+// returns when the kernels before it have completed and their writes are visible.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// cluster = 0: the kernel has its own cluster size, or none
+template <typename... P, typename... A>
+inline cudaError_t launch_serialized(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, unsigned cluster, cudaStream_t s,
+                                     const A&... args) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ---- clusters and CTA pairs ---------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;

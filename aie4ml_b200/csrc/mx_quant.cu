@@ -65,6 +65,8 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(QuantArgs g) {
     const int valid = (int)max(0LL, min(8LL, g.cols - col));
     reinterpret_cast<uint32_t*>(sc)[threadIdx.x] = 0u;
     __syncthreads();
+    grid_wait();
+    grid_release();
     const int code_bytes = (valid + 1) >> 1;      // an odd last column leaves a zero in the high nibble
     const bool any = row0 + warp * ROWS_PER_WARP < g.rows;
 #pragma unroll 4
@@ -120,6 +122,8 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(DequantArgs g) {
     const long long row0 = (long long)by * ROWS;
     const long long col = (long long)bx * COLS + lane * 8;
     const int valid = (int)max(0LL, min(8LL, g.cols - col));
+    grid_wait();
+    grid_release();
     if (valid == 0) return;
 #pragma unroll 4
     for (int i = 0; i < ROWS_PER_WARP; ++i) {
@@ -175,9 +179,8 @@ int a4c_launch_quantize_mx(const void* x, int kind, long long ldx, uint8_t* code
     g.x = x; g.ldx = ldx; g.codes = codes; g.ldc_bytes = ldc / 2; g.scales = scales; g.rows = rows; g.cols = cols;
     g.across = tiles_across(cols);
     g.vec = ((uintptr_t)x & 15u) == 0 && (ldx * esz) % 16 == 0;
-    if (kind == KIND_BF16) quantize_kernel<KIND_BF16><<<grid, THREADS, 0, stream>>>(g);
-    else quantize_kernel<KIND_F32><<<grid, THREADS, 0, stream>>>(g);
-    return cudaGetLastError() == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
+    const cudaError_t e = launch_serialized(kind == KIND_BF16 ? quantize_kernel<KIND_BF16> : quantize_kernel<KIND_F32>, grid, THREADS, 0, 0, stream, g);
+    return e == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
 }
 
 int a4c_launch_dequantize_mx(const uint8_t* codes, long long ldc, const uint8_t* scales, void* y, int kind, long long ldy,
@@ -189,7 +192,6 @@ int a4c_launch_dequantize_mx(const uint8_t* codes, long long ldc, const uint8_t*
     g.codes = codes; g.ldc_bytes = ldc / 2; g.scales = scales; g.y = y; g.ldy = ldy; g.rows = rows; g.cols = cols;
     g.across = tiles_across(cols);
     g.vec = ((uintptr_t)y & 15u) == 0 && (ldy * esz) % 16 == 0;
-    if (kind == KIND_BF16) dequantize_kernel<KIND_BF16><<<grid, THREADS, 0, stream>>>(g);
-    else dequantize_kernel<KIND_F32><<<grid, THREADS, 0, stream>>>(g);
-    return cudaGetLastError() == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
+    const cudaError_t e = launch_serialized(kind == KIND_BF16 ? dequantize_kernel<KIND_BF16> : dequantize_kernel<KIND_F32>, grid, THREADS, 0, 0, stream, g);
+    return e == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
 }
