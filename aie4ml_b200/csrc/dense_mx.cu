@@ -14,9 +14,11 @@
 // rank sends its partial sums to the rank that finishes the row (distributed shared memory), which adds them in rank order,
 // so the result does not depend on timing and no workspace exists.
 //
-// One tile per CTA: warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue.  A stage is 256 values of K: 128-byte
-// swizzled rows of codes and the scale tiles, which tcgen05.cp moves on to TMEM ahead of the stage's MMAs (the tensor
-// pipe takes both in issue order).  Every wait is bounded.
+// One tile per CTA: warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue, of which warp 2 first moves the scales on to
+// TMEM (tcgen05.cp; a set of columns per stage, so it runs ahead of the MMAs; copies issued by the MMA thread run in turn with
+// its MMAs and held a stage at 0.6 us).  A stage is 256 values of K: 128-byte swizzled rows of codes and the scale tiles.
+// A CTA runs all of its code once, so unrolled code costs its way out of memory: the epilogue converts 16 rows at a time.
+// Every wait is bounded.
 #include <cuda.h>
 
 #include "a4c_common.cuh"
@@ -34,6 +36,7 @@ constexpr int W_BYTES = BN * BK / 2;
 constexpr int SF_BYTES = 2 * mx::TILE_BYTES;  // scales of 128 rows x 256 values
 constexpr int NUM_THREADS = 192;
 constexpr int MAX_STAGES = 12;
+constexpr int MAX_GATED_STAGES = 10;
 constexpr int MAX_SPLIT = 8;                  // portable cluster size
 constexpr int SPLIT_T = 32;                   // most rows per tile when the reduction is split
 constexpr int SMEM_BUDGET = 200 * 1024;
@@ -42,7 +45,7 @@ constexpr size_t ONE_PER_SM = 116 * 1024;
 struct Tail {
     uint64_t full[MAX_STAGES];
     uint64_t empty[MAX_STAGES];
-    uint64_t moved[MAX_STAGES];      // the stage's A scales lie in the first column
+    uint64_t scaled[MAX_STAGES];     // the stage's scales lie in tensor memory
     uint64_t done;
     uint32_t tmem_base;
     volatile int abort_flag;
@@ -59,11 +62,11 @@ struct Args {
     int k_tiles;                     // scale tiles across K
     int num_kb;                      // stages of the whole reduction
     int t;                           // rows of A per tile: 16, 32, 64 or 128
-    int split;                       // CTAs per tile (cluster size)
+    int split, log_split;            // CTAs per tile (cluster size), a power of two
     int num_n_tiles;
     int stages, stage_bytes;         // the partial sums of a split reduction lie behind the stages
     int part_bytes;
-    int out_kind, act;
+    int act;
     uint32_t idesc;
     int* status;
 };
@@ -72,54 +75,72 @@ __device__ __forceinline__ void st_cluster(uint32_t local, uint32_t rank, float 
     asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(mx::map_to_cta(local, rank)), "f"(v) : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
+    uint32_t a[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]),
+          "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(a[i]);
+}
+
 // One value of row m and feature n (this lane's), complete over K; the 32 lanes of a warp hold 32 neighbouring
 // features, which for an MXFP4 output are one block.  Called by whole warps with the same m.
+template <int OUT>
 __device__ __forceinline__ void store_value(const Args& g, long long m, int n, float v) {
-    if (g.out_kind == mx::KIND_BF16) {
+    if (OUT == mx::KIND_BF16) {
         if (n < g.N) reinterpret_cast<__nv_bfloat16*>(g.Y)[m * g.ldy + n] = __float2bfloat16_rn(v);
-    } else if (g.out_kind == mx::KIND_F32) {
+    } else if (OUT == mx::KIND_F32) {
         if (n < g.N) reinterpret_cast<float*>(g.Y)[m * g.ldy + n] = v;
     } else {
         const int lane = threadIdx.x & 31;
         const int n0 = n - lane;
         if (n >= g.N) v = 0.0f;
         const uint32_t s = mx::scale_code(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu));
-        const float q[8] = {v * mx::inverse_scale(s == 255u ? 0u : s), 0, 0, 0, 0, 0, 0, 0};
-        uint32_t w = s == 255u ? 0u : (mx::pack_e2m1(q) & 15u) << (4 * (lane & 7));
+        uint32_t w = s == 255u ? 0u : mx::one_e2m1(v * mx::inverse_scale(s)) << (4 * (lane & 7));
         w |= __shfl_xor_sync(0xFFFFFFFFu, w, 1);
         w |= __shfl_xor_sync(0xFFFFFFFFu, w, 2);
         w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
-        if (n0 < g.N) {
-            uint8_t* dst = reinterpret_cast<uint8_t*>(g.Y) + (m * g.ldy + n0) / 2;
-            const int bytes = (min(32, g.N - n0) + 1) >> 1;
-            // lane 8 j holds the word of features 8 j .. 8 j + 7
-            if ((lane & 7) == 0) {
-                const int b0 = lane >> 1;
-                if (b0 + 4 <= bytes) *reinterpret_cast<uint32_t*>(dst + b0) = w;
-                else for (int b = b0; b < bytes; ++b) dst[b] = (uint8_t)(w >> (8 * (b - b0)));
-            }
-            if (lane == 0) g.ys[mx::scale_offset(m, n0 >> 5, g.y_across)] = (uint8_t)s;
-        } else if ((n0 >> 5) < (int)g.y_across * mx::TILE_BLOCKS && lane == 0) {
-            g.ys[mx::scale_offset(m, n0 >> 5, g.y_across)] = 0;   // places beyond the tensor
+        uint8_t* dst = reinterpret_cast<uint8_t*>(g.Y) + (m * g.ldy + n0) / 2;
+        const int bytes = (min(32, g.N - n0) + 1) >> 1;       // <= 0 for a block beyond the row's end, whose scale is 0
+        // lane 8 j holds the word of features 8 j .. 8 j + 7
+        if ((lane & 7) == 0) {
+            const int b0 = lane >> 1;
+            if (b0 + 4 <= bytes) *reinterpret_cast<uint32_t*>(dst + b0) = w;
+            else for (int b = b0; b < bytes; ++b) dst[b] = (uint8_t)(w >> (8 * (b - b0)));
         }
+        if (lane == 0) g.ys[mx::scale_offset(m, n0 >> 5, g.y_across)] = (uint8_t)s;
     }
 }
 
-template <bool GATED>
-__device__ __forceinline__ float finish_value(const Args& g, float a, float u, float ba, float bu) {
-    a += ba;
-    if (GATED) return mx::activate(a, g.act) * (u + bu);
-    return g.act == mx::ACT_RELU && a < 0.0f ? 0.0f : a;
+// N values (of as many rows) of this lane's feature: bias, activation, product
+template <bool GATED, int N>
+__device__ __forceinline__ void finish_values(const Args& g, float* a, const float* u, float ba, float bu) {
+    mx::f2 v[(N + 1) / 2];
+#pragma unroll
+    for (int i = 0; i < (N + 1) / 2; ++i) v[i] = mx::add2(mx::pack2(a[2 * i], N > 1 ? a[2 * i + 1] : 0.0f), mx::both(ba));
+    if (GATED || g.act == mx::ACT_RELU) mx::activate_pairs<(N + 1) / 2>(v, GATED ? g.act : mx::ACT_RELU);
+#pragma unroll
+    for (int i = 0; i < (N + 1) / 2; ++i) {
+        float lo, hi;
+        mx::unpack2(v[i], lo, hi);
+        a[2 * i] = GATED ? lo * (u[2 * i] + bu) : lo;
+        if (N > 1) a[2 * i + 1] = GATED ? hi * (u[2 * i + 1] + bu) : hi;
+    }
 }
 
-template <bool GATED>
+template <bool GATED, int OUT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                 const __grid_constant__ CUtensorMap map_u, Args g) {
     constexpr int NW = GATED ? 2 : 1;
     constexpr int SF_COLS = NW * 8 + 8;               // TMEM columns of one stage's scales: W (each), then A
     constexpr int SF0 = NW * MAX_T;                   // after the accumulators
-    constexpr int TMEM_COLS = GATED ? 512 : 256;      // a power of two >= SF0 + 2 * SF_COLS
+    constexpr int TMEM_COLS = 512;
+    static_assert(SF0 + (GATED ? MAX_GATED_STAGES : MAX_STAGES) * SF_COLS <= TMEM_COLS, "a set of scale columns per stage");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     float* part = reinterpret_cast<float*>(smem + (size_t)g.stages * g.stage_bytes);
@@ -156,7 +177,7 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     };
     const int ahead = min(g.stages, kb1 - kb0);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < g.stages; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); mbar_init(&tail->moved[s], 1); }
+        for (int s = 0; s < g.stages; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); mbar_init(&tail->scaled[s], 1); }
         mbar_init(&tail->done, 1);
         tail->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -194,31 +215,21 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             uint32_t phase = 0;
             bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb) {
-                ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 152) &&
-                     (sf_row == 0 || mbar_wait(&tail->moved[stage], phase, abort_flag, g.status, 154));
+                ok = mbar_wait(&tail->scaled[stage], phase, abort_flag, g.status, 152) &&
+                     mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 154);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t s = smem_u32(smem) + (uint32_t)(stage * g.stage_bytes);
-                const uint32_t f = s + (uint32_t)(g.stage_bytes - (NW + 1) * SF_BYTES);
                 const int steps = min(4, (g.K - kb * BK + 63) / 64);   // MMAs of 64 values; beyond K nothing is read
-                const uint32_t sf = tmem_base + (uint32_t)(SF0 + ((kb - kb0) & 1) * SF_COLS);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {                          // scale tiles of 128 values of K
-                    if (steps <= 2 * h) break;
-#pragma unroll
-                    for (int o = 0; o < NW + 1; ++o)
-                        mx::copy_scales(sf + (uint32_t)(o * 8 + h * 4), mx::make_scale_desc(f + (uint32_t)(o * SF_BYTES + h * mx::TILE_BYTES)));
-                }
-                const uint64_t adesc = make_smem_desc(s + NW * W_BYTES);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (k >= steps) break;
+                const uint32_t sf = tmem_base + (uint32_t)(SF0 + stage * SF_COLS);
+                const uint64_t wdesc = make_smem_desc(s), adesc = make_smem_desc(s + NW * W_BYTES);
+#pragma unroll 1
+                for (int k = 0; k < steps; ++k) {
                     const uint32_t idesc = g.idesc | mx::sf_bits(k & 1);
 #pragma unroll
                     for (int o = 0; o < NW; ++o)
-                        mx::umma(tmem_base + (uint32_t)(o * MAX_T), make_smem_desc(s + o * W_BYTES) + (uint64_t)(k * 2), adesc + (uint64_t)(k * 2),
-                                 idesc, sf + (uint32_t)(o * 8 + (k >> 1) * 4), sf + (uint32_t)(NW * 8 + (k >> 1) * 4),
-                                 (uint32_t)(kb != kb0 || k != 0));
+                        mx::umma(tmem_base + (uint32_t)(o * MAX_T), wdesc + (uint64_t)(o * (W_BYTES >> 4) + k * 2), adesc + (uint64_t)(k * 2), idesc,
+                                 sf + (uint32_t)(o * 8 + (k >> 1) * 4), sf + (uint32_t)(NW * 8 + (k >> 1) * 4), (uint32_t)(kb != kb0 || k != 0));
                 }
                 umma_commit(&tail->empty[stage]);
                 if (++stage == g.stages) { stage = 0; phase ^= 1u; }
@@ -226,21 +237,32 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (ok) umma_commit(&tail->done);
         }
         __syncwarp();
-    } else if (warp == 2 && sf_row != 0) {
+    } else if (warp == 2) {
+        // a stage's columns were last read by the MMAs whose completion let the stage be filled again
         int stage = 0;
         uint32_t phase = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 155)) break;
-            uint32_t* f = reinterpret_cast<uint32_t*>(smem + (size_t)(stage + 1) * g.stage_bytes - SF_BYTES) + lane * 4;
-            const bool two = g.k_tiles - 2 * kb > 1;
-            f[0] = f[sf_row];
-            if (two) f[mx::TILE_BYTES / 4] = f[mx::TILE_BYTES / 4 + sf_row];
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            uint8_t* f = smem + (size_t)(stage + 1) * g.stage_bytes - (NW + 1) * SF_BYTES;
+            const int halves = min(2, g.k_tiles - 2 * kb);             // scale tiles of 128 values of K
+            if (sf_row != 0) {
+                uint32_t* fa = reinterpret_cast<uint32_t*>(f + NW * SF_BYTES) + lane * 4;
+                for (int h = 0; h < halves; ++h) fa[h * (mx::TILE_BYTES / 4)] = fa[h * (mx::TILE_BYTES / 4) + sf_row];
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
+            if (lane == 0) {
+                tc_fence_after();
+                const uint32_t sf = tmem_base + (uint32_t)(SF0 + stage * SF_COLS);
+#pragma unroll
+                for (int o = 0; o < NW + 1; ++o)
+                    for (int h = 0; h < halves; ++h)
+                        mx::copy_scales(sf + (uint32_t)(o * 8 + h * 4), mx::make_scale_desc(smem_u32(f) + (uint32_t)(o * SF_BYTES + h * mx::TILE_BYTES)));
+                umma_commit(&tail->scaled[stage]);
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tail->moved[stage]);
             if (++stage == g.stages) { stage = 0; phase ^= 1u; }
         }
-        __syncwarp();
     }
 
     const int quad = warp & 3;
@@ -261,47 +283,40 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     if (g.split == 1) {
         if (ok) {
 #pragma unroll 1
-            for (int c = 0; c < rows; c += 32) {
-                uint32_t a[32], u[32];
-                tmem_ld32(taddr + (uint32_t)c, a);
-                if (GATED) tmem_ld32(taddr + (uint32_t)(MAX_T + c), u);
+            for (int c = 0; c < rows; c += 16) {
+                float a[16], u[16];
+                tmem_ld16(taddr + (uint32_t)c, a);
+                if (GATED) tmem_ld16(taddr + (uint32_t)(MAX_T + c), u);
+                finish_values<GATED, 16>(g, a, u, ba, bu);
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (c + i < rows)
-                        store_value(g, m0 + c + i, n,
-                                    finish_value<GATED>(g, __uint_as_float(a[i]), GATED ? __uint_as_float(u[i]) : 0.0f, ba, bu));
+                for (int i = 0; i < 16; ++i)
+                    if (c + i < rows) store_value<OUT>(g, m0 + c + i, n, a[i]);
             }
         }
     } else {
         // row r is finished by rank r mod split; part[from][r / split][projection][feature] there
-        const int per = g.t / g.split;
+        const int per = g.t >> g.log_split;
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // every rank has started
         if (ok) {
             const uint32_t base = smem_u32(part) + (uint32_t)((int)rank * per * NW * BN + nl) * 4u;
 #pragma unroll 1
             for (int c = 0; c < rows; c += 16)
-#pragma unroll
+#pragma unroll 1
                 for (int o = 0; o < NW; ++o) {
-                    uint32_t a[16];
-                    asm volatile(
-                        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]),
-                          "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])
-                        : "r"(taddr + (uint32_t)(o * MAX_T + c)));
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    float a[16];
+                    tmem_ld16(taddr + (uint32_t)(o * MAX_T + c), a);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int r = c + i;
-                        if (r < rows)
-                            st_cluster(base + (uint32_t)((r / g.split) * NW + o) * (BN * 4u), (uint32_t)(r & (g.split - 1)), __uint_as_float(a[i]));
-                    }
+                    for (int i = 0; i < 16; ++i)
+                        if (c + i < rows)
+                            st_cluster(base + (uint32_t)(((c + i) >> g.log_split) * NW + o) * (BN * 4u), (uint32_t)((c + i) & (g.split - 1)), a[i]);
                 }
         }
         __syncwarp();
         mx::cluster_sync_all();          // all partial sums have arrived
         if (warp >= 2) {
-            for (int r = (int)rank; r < rows; r += g.split) {
-                const float* p = part + (r / g.split) * NW * BN + nl;
+            const float* p = part + nl;
+#pragma unroll 1
+            for (int r = (int)rank; r < rows; r += g.split, p += NW * BN) {
                 float a = 0.0f, u = 0.0f;
 #pragma unroll
                 for (int q = 0; q < MAX_SPLIT; ++q)
@@ -309,7 +324,8 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         a += p[q * per * NW * BN];
                         if (GATED) u += p[q * per * NW * BN + BN];
                     }
-                if (ok) store_value(g, m0 + r, n, finish_value<GATED>(g, a, u, ba, bu));
+                finish_values<GATED, 1>(g, &a, &u, ba, bu);
+                if (ok) store_value<OUT>(g, m0 + r, n, a);
             }
         }
     }
@@ -327,13 +343,12 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
 }
 
-template <bool GATED>
-cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mw, const CUtensorMap& mu, const Args& g, unsigned grid, size_t smem,
-                   cudaStream_t s) {
+template <bool GATED, int OUT>
+cudaError_t launch(const CUtensorMap* m, const Args& g, unsigned grid, size_t smem, cudaStream_t s) {
     static tc::SmemOptIn opt_in;
-    const cudaError_t e = opt_in.ensure(dense_mx_kernel<GATED>, SMEM_BUDGET + 16 * 1024);
+    const cudaError_t e = opt_in.ensure(dense_mx_kernel<GATED, OUT>, SMEM_BUDGET + 16 * 1024);
     if (e != cudaSuccess) return e;
-    return mx::launch_serialized(dense_mx_kernel<GATED>, grid, NUM_THREADS, smem, (unsigned)g.split, s, ma, mw, mu, g);
+    return mx::launch_serialized(dense_mx_kernel<GATED, OUT>, grid, NUM_THREADS, smem, (unsigned)g.split, s, m[0], m[1], m[2], g);
 }
 
 }  // namespace
@@ -350,7 +365,7 @@ int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stre
     g.Y = d.y; g.ldy = d.ldy; g.ys = d.ys; g.y_across = mx::tiles_across(d.N);
     g.M = d.M; g.N = d.N; g.K = d.K; g.k_tiles = (int)mx::tiles_across(d.K);
     g.num_kb = (d.K + BK - 1) / BK;
-    g.out_kind = d.out_kind; g.act = d.act; g.status = status_word;
+    g.act = d.act; g.status = status_word;
     g.num_n_tiles = (d.N + BN - 1) / BN;
     g.t = d.M > 64 ? 128 : d.M > 32 ? 64 : d.M > 16 ? 32 : 16;
     auto tiles_of = [&](int t) { return (d.M + t - 1) / t * g.num_n_tiles; };
@@ -360,11 +375,12 @@ int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stre
     const long long tiles = tiles_of(g.t);
     g.split = 1;
     while (g.split < MAX_SPLIT && g.t <= SPLIT_T && tiles * g.split * 2 <= sms && g.split * 2 <= g.num_kb) g.split *= 2;
+    g.log_split = g.split == 1 ? 0 : g.split == 2 ? 1 : g.split == 4 ? 2 : 3;
     g.idesc = mx::make_idesc(BN, g.t);
     g.stage_bytes = nw * W_BYTES + g.t * (BK / 2) + (nw + 1) * SF_BYTES;
     const int need = (g.num_kb + g.split - 1) / g.split;
     int stages = (SMEM_BUDGET - (g.split > 1 ? nw * g.t * BN * 4 : 0)) / g.stage_bytes;
-    if (stages > MAX_STAGES) stages = MAX_STAGES;
+    if (stages > (gated ? MAX_GATED_STAGES : MAX_STAGES)) stages = gated ? MAX_GATED_STAGES : MAX_STAGES;
     if (need < stages) stages = need;
     g.stages = stages;
     g.part_bytes = g.split > 1 ? nw * g.t * BN * 4 : 0;
@@ -372,11 +388,17 @@ int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stre
     // More than half of an SM's shared memory, so that one CTA lives on an SM at a time: the ranks of a cluster wait for
     // one another while they hold tensor memory, and two clusters that shared SMs could each wait for the other's.
     if (smem < ONE_PER_SM) smem = ONE_PER_SM;
-    CUtensorMap ma, mw, mu;
-    if (!mx::make_code_map(&ma, d.a, d.M, d.K, d.lda, g.t) || !mx::make_code_map(&mw, d.w, d.N, d.K, d.ldw, BN) ||
-        !mx::make_code_map(&mu, gated ? d.wu : d.w, d.N, d.K, gated ? d.ldu : d.ldw, BN))
-        return A4C_ERR_CUDA;
+    CUtensorMap m[3];
+    if (!mx::make_code_map(&m[0], d.a, d.M, d.K, d.lda, g.t) || !mx::make_code_map(&m[1], d.w, d.N, d.K, d.ldw, BN)) return A4C_ERR_CUDA;
+    m[2] = m[1];
+    if (gated && !mx::make_code_map(&m[2], d.wu, d.N, d.K, d.ldu, BN)) return A4C_ERR_CUDA;
     const unsigned grid = (unsigned)(tiles * g.split);
-    const cudaError_t err = gated ? launch<true>(ma, mw, mu, g, grid, smem, stream) : launch<false>(ma, mw, mu, g, grid, smem, stream);
+    cudaError_t err;
+    if (gated)
+        err = d.out_kind == mx::KIND_BF16 ? launch<true, mx::KIND_BF16>(m, g, grid, smem, stream)
+              : d.out_kind == mx::KIND_F32 ? launch<true, mx::KIND_F32>(m, g, grid, smem, stream) : launch<true, mx::KIND_MX>(m, g, grid, smem, stream);
+    else
+        err = d.out_kind == mx::KIND_BF16 ? launch<false, mx::KIND_BF16>(m, g, grid, smem, stream)
+              : d.out_kind == mx::KIND_F32 ? launch<false, mx::KIND_F32>(m, g, grid, smem, stream) : launch<false, mx::KIND_MX>(m, g, grid, smem, stream);
     return err == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
 }

@@ -53,6 +53,14 @@ __device__ __forceinline__ uint32_t pack_e2m1(const float* v) {
         : "=r"(w) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return w;
 }
+// one value; the codes' byte stands in all four
+__device__ __forceinline__ uint32_t one_e2m1(float v) {
+    uint32_t w;
+    asm("{\n\t.reg .b8 b0;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "mov.b32 %0, {b0, b0, b0, b0};\n\t}" : "=r"(w) : "f"(v), "f"(0.0f));
+    return w & 15u;
+}
 // Eight E2M1 codes -> float (exact)
 __device__ __forceinline__ void unpack_e2m1(uint32_t w, float* v) {
     uint32_t h[4];
