@@ -7,7 +7,7 @@
 // takes eight neighbouring columns, so a block is four lanes and its maximum two shuffles; a warp takes 256 columns of a
 // row.  A CTA takes 128 rows x 256 columns: exactly two scale tiles, which it gathers in shared memory and writes out
 // whole (places beyond the tensor as 0), because single scale bytes 16 bytes apart would touch every 32-byte sector of
-// the scale array many times.
+// the scale array many times.  Where that leaves SMs idle a CTA takes 32 rows, a quarter of each tile: a word in 16 bytes.
 #include "a4c_common.cuh"
 #include "a4c_kernels.h"
 #include "mx_common.cuh"
@@ -16,10 +16,9 @@ namespace {
 
 using namespace mx;
 
-constexpr int ROWS = TILE_ROWS;      // rows per CTA
 constexpr int COLS = 256;            // columns per CTA: 32 lanes x 8
 constexpr int THREADS = 256;
-constexpr int ROWS_PER_WARP = ROWS / (THREADS / 32);
+constexpr int WARPS = THREADS / 32;
 
 struct QuantArgs {
     const void* x; long long ldx;
@@ -30,79 +29,103 @@ struct QuantArgs {
     int vec;                         // x can be read in 16-byte pieces
 };
 
+// Eight neighbouring values as they lie in memory; those beyond `valid` read as zero
+template <int KIND> struct Raw { uint32_t w[KIND == KIND_BF16 ? 4 : 8]; };
+
 template <int KIND>
-__device__ __forceinline__ void load8(const void* base, long long idx, int valid, bool vec, float* v) {
+__device__ __forceinline__ Raw<KIND> load8(const void* base, long long idx, int valid, bool vec) {
+    Raw<KIND> r;
     if (KIND == KIND_BF16) {
         const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + idx;
-        if (vec && valid >= 8) {
+        if (vec && valid == 8) {
             const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p));
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+            r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < valid ? __uint_as_float((uint32_t)p[i] << 16) : 0.0f;
+            for (int i = 0; i < 4; ++i)
+                r.w[i] = (2 * i < valid ? (uint32_t)p[2 * i] : 0u) | (2 * i + 1 < valid ? (uint32_t)p[2 * i + 1] << 16 : 0u);
         }
     } else {
-        const float* p = reinterpret_cast<const float*>(base) + idx;
-        if (vec && valid >= 8) {
-            const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(base) + idx;
+        if (vec && valid == 8) {
+            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p)), b = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
+            r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+            r.w[4 % (sizeof(r.w) / 4)] = b.x; r.w[5 % (sizeof(r.w) / 4)] = b.y; r.w[6 % (sizeof(r.w) / 4)] = b.z; r.w[7 % (sizeof(r.w) / 4)] = b.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < valid ? p[i] : 0.0f;
+            for (int i = 0; i < (int)(sizeof(r.w) / 4); ++i) r.w[i] = i < valid ? p[i] : 0u;
         }
+    }
+    return r;
+}
+template <int KIND>
+__device__ __forceinline__ void values_of(const Raw<KIND>& r, float* v) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(r.w) / 4); ++i) {
+        if (KIND == KIND_BF16) { v[2 * i] = __uint_as_float(r.w[i] << 16); v[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u); }
+        else v[i] = __uint_as_float(r.w[i]);
     }
 }
 
-template <int KIND>
+constexpr int BATCH = 4;             // rows whose loads a warp issues before it converts any (the stores between would hold them back)
+
+// QUARTERS x 32 rows per CTA: 4 (whole scale tiles) or 1
+template <int KIND, int QUARTERS>
 __global__ void __launch_bounds__(THREADS) quantize_kernel(QuantArgs g) {
-    __shared__ __align__(16) uint8_t sc[2 * TILE_BYTES];
+    constexpr int ROWS = QUARTERS * 32;
+    __shared__ __align__(16) uint8_t sc[2 * TILE_BYTES / 4 * QUARTERS];   // [tile][row % 32][quarter][block]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned by = blockIdx.x / g.grid_cols, bx = blockIdx.x - by * g.grid_cols;
     const long long row0 = (long long)by * ROWS;
     const long long col = (long long)bx * COLS + lane * 8;
     const int valid = (int)max(0LL, min(8LL, g.cols - col));
-    reinterpret_cast<uint32_t*>(sc)[threadIdx.x] = 0u;
+    if (threadIdx.x < 64 * QUARTERS) reinterpret_cast<uint32_t*>(sc)[threadIdx.x] = 0u;
     __syncthreads();
     grid_wait();
     grid_release();
     const int code_bytes = (valid + 1) >> 1;      // an odd last column leaves a zero in the high nibble
-    const bool any = row0 + warp * ROWS_PER_WARP < g.rows;
-#pragma unroll 4
-    for (int i = 0; any && i < ROWS_PER_WARP; ++i) {
-        const int r = warp * ROWS_PER_WARP + i;
-        const long long row = row0 + r;
-        const bool live = row < g.rows;
-        float v[8];
-        load8<KIND>(g.x, live ? row * g.ldx + col : 0, live ? valid : 0, g.vec != 0, v);
-        uint32_t top = 0;
+    const int count = (int)max(0LL, min((long long)ROWS, g.rows - row0));
+    for (int first = warp; first < count; first += BATCH * WARPS) {
+        Raw<KIND> raw[BATCH];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        const uint32_t s = scale_code(top);
-        const float inv = inverse_scale(s == 255u ? 0u : s);
+        for (int j = 0; j < BATCH; ++j)
+            raw[j] = load8<KIND>(g.x, (row0 + first + j * WARPS) * g.ldx + col, first + j * WARPS < count ? valid : 0, g.vec != 0);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= inv;
-        const uint32_t w = s == 255u ? 0u : pack_e2m1(v);
-        if (live && valid > 0) {
-            uint8_t* dst = g.codes + row * g.ldc_bytes + (col >> 1);
-            if (valid == 8) *reinterpret_cast<uint32_t*>(dst) = w;
-            else for (int k = 0; k < code_bytes; ++k) dst[k] = (uint8_t)(w >> (8 * k));
-            if ((lane & 3) == 0) {
-                const int b = lane >> 2;          // block within the CTA's eight
-                sc[(b >> 2) * TILE_BYTES + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = (uint8_t)s;
+        for (int j = 0; j < BATCH; ++j) {
+            const int r = first + j * WARPS;
+            if (r >= count) break;                // the same for the whole warp
+            float v[8];
+            values_of(raw[j], v);
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            const uint32_t s = scale_code(top);
+            const float inv = inverse_scale(s == 255u ? 0u : s);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= inv;
+            const uint32_t w = s == 255u ? 0u : pack_e2m1(v);
+            if (valid > 0) {
+                uint8_t* dst = g.codes + (row0 + r) * g.ldc_bytes + (col >> 1);
+                if (valid == 8) *reinterpret_cast<uint32_t*>(dst) = w;
+                else for (int k = 0; k < code_bytes; ++k) dst[k] = (uint8_t)(w >> (8 * k));
+                if ((lane & 3) == 0) {
+                    const int b = lane >> 2;      // block within the CTA's eight
+                    sc[(((b >> 2) * 32 + (r & 31)) * QUARTERS + (r >> 5)) * 4 + (b & 3)] = (uint8_t)s;
+                }
             }
         }
     }
     __syncthreads();
-    // 64 pieces of 16 bytes; the second tile exists when the tensor reaches into it
+    // a thread per tile and row % 32; the second tile exists when the tensor reaches into it
     if (threadIdx.x < 64) {
         const long long tile = (long long)bx * 2 + (threadIdx.x >> 5);
-        if (tile < g.across)
-            reinterpret_cast<uint4*>(g.scales + ((long long)by * g.across + tile) * TILE_BYTES)[threadIdx.x & 31] =
-                reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+        if (tile < g.across) {
+            uint8_t* dst = g.scales + ((row0 / TILE_ROWS) * g.across + tile) * TILE_BYTES + (threadIdx.x & 31) * 16;
+            if (QUARTERS == 4) *reinterpret_cast<uint4*>(dst) = reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+            else reinterpret_cast<uint32_t*>(dst)[by & 3] = reinterpret_cast<const uint32_t*>(sc)[threadIdx.x];
+        }
     }
 }
 
@@ -115,8 +138,9 @@ struct DequantArgs {
     int vec;                         // y can be written in 16-byte pieces
 };
 
-template <int KIND>
+template <int KIND, int QUARTERS>
 __global__ void __launch_bounds__(THREADS) dequantize_kernel(DequantArgs g) {
+    constexpr int ROWS = QUARTERS * 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned by = blockIdx.x / g.grid_cols, bx = blockIdx.x - by * g.grid_cols;
     const long long row0 = (long long)by * ROWS;
@@ -125,47 +149,70 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(DequantArgs g) {
     grid_wait();
     grid_release();
     if (valid == 0) return;
-#pragma unroll 4
-    for (int i = 0; i < ROWS_PER_WARP; ++i) {
-        const long long row = row0 + warp * ROWS_PER_WARP + i;
-        if (row >= g.rows) return;
-        const uint8_t* src = g.codes + row * g.ldc_bytes + (col >> 1);
-        uint32_t w = 0;
-        if (valid == 8) w = __ldcs(reinterpret_cast<const uint32_t*>(src));
-        else for (int k = 0; k < (valid + 1) >> 1; ++k) w |= (uint32_t)src[k] << (8 * k);
-        const float scale = scale_value(__ldg(g.scales + scale_offset(row, col >> 5, g.across)));
-        float v[8];
-        unpack_e2m1(w, v);
+    const int count = (int)max(0LL, min((long long)ROWS, g.rows - row0));
+    for (int first = warp; first < count; first += BATCH * WARPS) {
+        uint32_t code[BATCH];
+        uint8_t sc[BATCH];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= scale;
-        if (KIND == KIND_BF16) {
-            uint16_t* dst = reinterpret_cast<uint16_t*>(g.y) + row * g.ldy + col;
-            const uint4 q = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-            if (g.vec && valid == 8) __stcs(reinterpret_cast<uint4*>(dst), q);
-            else {
-                const uint32_t p[4] = {q.x, q.y, q.z, q.w};
+        for (int j = 0; j < BATCH; ++j) {
+            const int r = first + j * WARPS;
+            code[j] = 0;
+            sc[j] = 0;
+            if (r >= count) continue;
+            const uint8_t* src = g.codes + (row0 + r) * g.ldc_bytes + (col >> 1);
+            if (valid == 8) code[j] = __ldcs(reinterpret_cast<const uint32_t*>(src));
+            else for (int k = 0; k < (valid + 1) >> 1; ++k) code[j] |= (uint32_t)src[k] << (8 * k);
+            sc[j] = __ldg(g.scales + scale_offset(row0 + r, col >> 5, g.across));
+        }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) if (k < valid) dst[k] = (uint16_t)(p[k >> 1] >> (16 * (k & 1)));
-            }
-        } else {
-            float* dst = reinterpret_cast<float*>(g.y) + row * g.ldy + col;
-            if (g.vec && valid == 8) {
-                __stcs(reinterpret_cast<float4*>(dst), make_float4(v[0], v[1], v[2], v[3]));
-                __stcs(reinterpret_cast<float4*>(dst) + 1, make_float4(v[4], v[5], v[6], v[7]));
+        for (int j = 0; j < BATCH; ++j) {
+            const long long row = row0 + first + j * WARPS;
+            if (first + j * WARPS >= count) break;
+            const float scale = scale_value(sc[j]);
+            float v[8];
+            unpack_e2m1(code[j], v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= scale;
+            if (KIND == KIND_BF16) {
+                uint16_t* dst = reinterpret_cast<uint16_t*>(g.y) + row * g.ldy + col;
+                const uint4 q = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+                if (g.vec && valid == 8) __stcs(reinterpret_cast<uint4*>(dst), q);
+                else {
+                    const uint32_t p[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) if (k < valid) dst[k] = (uint16_t)(p[k >> 1] >> (16 * (k & 1)));
+                }
             } else {
+                float* dst = reinterpret_cast<float*>(g.y) + row * g.ldy + col;
+                if (g.vec && valid == 8) {
+                    __stcs(reinterpret_cast<float4*>(dst), make_float4(v[0], v[1], v[2], v[3]));
+                    __stcs(reinterpret_cast<float4*>(dst) + 1, make_float4(v[4], v[5], v[6], v[7]));
+                } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) if (k < valid) dst[k] = v[k];
+                    for (int k = 0; k < 8; ++k) if (k < valid) dst[k] = v[k];
+                }
             }
         }
     }
 }
 
-bool grid_of(long long rows, long long cols, unsigned& grid, unsigned& grid_cols) {
-    const long long gx = (cols - 1) / COLS + 1, gy = (rows - 1) / ROWS + 1;
+// CTAs of `quarters` x 32 rows; rows of the last scale tile beyond the tensor belong to somebody too
+bool grid_of(long long rows, long long cols, int& quarters, unsigned& grid, unsigned& grid_cols) {
+    const long long gx = (cols - 1) / COLS + 1, gy = (rows - 1) / TILE_ROWS + 1;
     if (gx > 2147483647LL / gy) return false;
-    grid = (unsigned)(gx * gy);
+    quarters = gx * gy < 2 * 148 ? 1 : 4;
+    grid = (unsigned)(gx * gy * (quarters == 1 ? 4 : 1));
     grid_cols = (unsigned)gx;
     return true;
+}
+
+template <int KIND>
+cudaError_t launch_quantize(const QuantArgs& g, int quarters, unsigned grid, cudaStream_t s) {
+    return launch_serialized(quarters == 1 ? quantize_kernel<KIND, 1> : quantize_kernel<KIND, 4>, grid, THREADS, 0, 0, s, g);
+}
+template <int KIND>
+cudaError_t launch_dequantize(const DequantArgs& g, int quarters, unsigned grid, cudaStream_t s) {
+    return launch_serialized(quarters == 1 ? dequantize_kernel<KIND, 1> : dequantize_kernel<KIND, 4>, grid, THREADS, 0, 0, s, g);
 }
 
 }  // namespace
@@ -173,25 +220,27 @@ bool grid_of(long long rows, long long cols, unsigned& grid, unsigned& grid_cols
 int a4c_launch_quantize_mx(const void* x, int kind, long long ldx, uint8_t* codes, long long ldc, uint8_t* scales,
                            long long rows, long long cols, cudaStream_t stream) {
     unsigned grid;
+    int quarters;
     QuantArgs g;
-    if (!grid_of(rows, cols, grid, g.grid_cols)) return A4C_ERR_TOO_LARGE;
+    if (!grid_of(rows, cols, quarters, grid, g.grid_cols)) return A4C_ERR_TOO_LARGE;
     const int esz = kind == KIND_BF16 ? 2 : 4;
     g.x = x; g.ldx = ldx; g.codes = codes; g.ldc_bytes = ldc / 2; g.scales = scales; g.rows = rows; g.cols = cols;
     g.across = tiles_across(cols);
     g.vec = ((uintptr_t)x & 15u) == 0 && (ldx * esz) % 16 == 0;
-    const cudaError_t e = launch_serialized(kind == KIND_BF16 ? quantize_kernel<KIND_BF16> : quantize_kernel<KIND_F32>, grid, THREADS, 0, 0, stream, g);
+    const cudaError_t e = kind == KIND_BF16 ? launch_quantize<KIND_BF16>(g, quarters, grid, stream) : launch_quantize<KIND_F32>(g, quarters, grid, stream);
     return e == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
 }
 
 int a4c_launch_dequantize_mx(const uint8_t* codes, long long ldc, const uint8_t* scales, void* y, int kind, long long ldy,
                              long long rows, long long cols, cudaStream_t stream) {
     unsigned grid;
+    int quarters;
     DequantArgs g;
-    if (!grid_of(rows, cols, grid, g.grid_cols)) return A4C_ERR_TOO_LARGE;
+    if (!grid_of(rows, cols, quarters, grid, g.grid_cols)) return A4C_ERR_TOO_LARGE;
     const int esz = kind == KIND_BF16 ? 2 : 4;
     g.codes = codes; g.ldc_bytes = ldc / 2; g.scales = scales; g.y = y; g.ldy = ldy; g.rows = rows; g.cols = cols;
     g.across = tiles_across(cols);
     g.vec = ((uintptr_t)y & 15u) == 0 && (ldy * esz) % 16 == 0;
-    const cudaError_t e = launch_serialized(kind == KIND_BF16 ? dequantize_kernel<KIND_BF16> : dequantize_kernel<KIND_F32>, grid, THREADS, 0, 0, stream, g);
+    const cudaError_t e = kind == KIND_BF16 ? launch_dequantize<KIND_BF16>(g, quarters, grid, stream) : launch_dequantize<KIND_F32>(g, quarters, grid, stream);
     return e == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
 }
