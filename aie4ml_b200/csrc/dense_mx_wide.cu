@@ -10,17 +10,17 @@
 // each CTA its own A rows', both CTAs all 256 weight rows'.
 //
 // Tensor memory: two accumulators of 256 columns and the scales of two stages (48 columns) are more than 512 columns, so the
-// accumulators overlap by 48 columns.  The epilogue empties those first and says so on a barrier of its own; the next
-// tile's MMAs wait for that and not for the whole tile.
+// accumulators overlap by 48 columns.  The epilogue first moves those to shared memory and says so on a barrier of its own;
+// the next tile's MMAs wait for that and not for the tile's arithmetic.
 //
 // The scale copies (tcgen05.cp) have a warp of their own, one stage ahead of the MMAs and tied to them by barriers: issued
 // by the MMA thread they run in turn with the MMAs, six copies of a stage costing 0.22 us on top of its 0.40 us of MMAs
 // (4096 x 16384 x 8192: 303 us; spread out between the MMAs 346 us; from their own warp 240 us, no copies at all 205 us).
 //
-// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2 scale copies (leader CTA), 3-10
-// epilogue in two groups of four, each half of the columns.  A lane holds one row, so an MXFP4 output block is 32 registers of one thread; rows go out through a
-// swizzled patch of shared memory per warp and TMA stores (directly from registers every 16 bytes of a row were an L2
-// request of their own).  Every wait is bounded.
+// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2 scale copies (leader CTA), 3-18 epilogue: two groups of four warps per
+// accumulator, each half of the columns, so that two tiles are converted at once.  A lane holds one row, so an MXFP4 output block
+// is 32 values of one thread; rows go out through a swizzled patch of shared memory per warp and TMA stores (directly from
+// registers every 16 bytes of a row were an L2 request of their own).  Every wait is bounded.
 #include <cuda.h>
 
 #include "a4c_common.cuh"
@@ -37,17 +37,18 @@ constexpr int BK = 256;
 constexpr int CODE_BYTES = 128 * BK / 2;      // 128 rows of a stage's codes
 constexpr int SF_BYTES = 2 * mx::TILE_BYTES;  // and of its scales
 constexpr int STAGE_BYTES = 2 * CODE_BYTES + 3 * SF_BYTES;
-constexpr int STAGES = 5;
+constexpr int STAGES = 4;
 constexpr int SF_COLS = 24;                   // A 8, weights 16
 constexpr int SF_SETS = 2;
 constexpr int TMEM_COLS = 512;
 constexpr int SF0 = TMEM_COLS - SF_SETS * SF_COLS;
 constexpr int ACC1 = SF0 - BN;                // second accumulator: columns ACC1 .. SF0
 constexpr int OVERLAP = BN - ACC1;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
 constexpr int EPI_WARP0 = 3;                   // first epilogue warp
 constexpr int NUM_THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
-constexpr int PATCH_BYTES = 32 * 128;           // per epilogue warp: 32 rows of a TMA store's box
+constexpr int PATCH_BYTES = 32 * 64;            // per epilogue warp: 32 rows of a TMA store's box
+constexpr int STASH_BYTES = OVERLAP * 128 * 4;  // per accumulator: the shared columns of this CTA's rows, [column][row]
 
 struct Tail {
     uint64_t full[STAGES];
@@ -59,7 +60,7 @@ struct Tail {
     uint32_t tmem_base;
     volatile int abort_flag;
 };
-constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * PATCH_BYTES + sizeof(Tail);
+constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * PATCH_BYTES + 2 * STASH_BYTES + sizeof(Tail);
 
 struct Args {
     const float* bias[2];
@@ -142,6 +143,21 @@ __device__ __forceinline__ void store_direct(const Args& g, long long row, int c
     }
 }
 
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* a) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]),
+          "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])
+        : "r"(taddr));
+}
+// waits for the loads issued so far; the registers pass through, so no use of them is scheduled ahead
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t* a) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
+                   "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15])
+                 :: "memory");
+}
+
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
                  :: "l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1) : "memory");
@@ -149,32 +165,32 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 }
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
-// adds the bias of 32 neighbouring columns from `col` on; columns beyond the row's end get none
+// adds the bias of 16 neighbouring columns from `col` on; columns beyond the row's end get none
 __device__ __forceinline__ void add_bias(mx::f2* v, const float* bias, int col, int cols) {
-    if (col + 32 <= cols && ((uintptr_t)bias & 15u) == 0) {
+    if (col + 16 <= cols && ((uintptr_t)bias & 15u) == 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const float4 b = __ldg(reinterpret_cast<const float4*>(bias + col) + i);
             v[2 * i] = mx::add2(v[2 * i], mx::pack2(b.x, b.y));
             v[2 * i + 1] = mx::add2(v[2 * i + 1], mx::pack2(b.z, b.w));
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 8; ++i)
             v[i] = mx::add2(v[i], mx::pack2(col + 2 * i < cols ? __ldg(bias + col + 2 * i) : 0.0f, col + 2 * i + 1 < cols ? __ldg(bias + col + 2 * i + 1) : 0.0f));
     }
 }
 
-// 32 finished neighbouring values of each lane's row, `half` 0 or 1 of 64 (called for both, `first` says which comes first)
-// -> output and, for MXFP4, the two scales of the 64; a block that lies beyond the row's end gets scale 0
+// 32 finished neighbouring values of each lane's row, `half` 0 and then 1 of 64 -> output and, for MXFP4, the two scales of the
+// 64; a block that lies beyond the row's end gets scale 0
 template <int OUT>
 __device__ __forceinline__ void store32(const Args& g, const CUtensorMap* map_y, uint8_t* patch, long long row0, int lane, int col, int half,
-                                        bool first, uint32_t& scales, mx::f2* v) {
+                                        uint32_t& scales, mx::f2* v) {
     const long long row = row0 + lane;
     constexpr int WORDS = Words<OUT>::value;
-    constexpr int BOX = OUT == mx::KIND_F32 ? 32 : 64;     // columns per TMA store: 128 bytes of bf16 or f32, 32 of MXFP4
+    constexpr int BOX = OUT == mx::KIND_F32 ? 16 : OUT == mx::KIND_BF16 ? 32 : 64;     // columns per TMA store: 64 bytes, or 32 of MXFP4
     const int col64 = col - 32 * half;
-    const bool boxed = g.tma_store && (BOX == 32 ? col : col64) + BOX <= g.N;
+    const bool boxed = g.tma_store && (OUT == mx::KIND_MX ? col64 + 64 : col + 32) <= g.N;
     if (OUT == mx::KIND_MX && col + 32 > g.N) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -183,29 +199,32 @@ __device__ __forceinline__ void store32(const Args& g, const CUtensorMap* map_y,
         }
     }
     uint32_t w[WORDS];
-    scales = (first ? 0u : scales) | to_words<OUT>(v, w) << (8 * half);
-    if (OUT == mx::KIND_MX && !first && row < g.M && (col64 >> 5) < (int)g.y_across * mx::TILE_BLOCKS)
+    scales = half == 0 ? to_words<OUT>(v, w) : scales | to_words<OUT>(v, w) << 8;
+    if (OUT == mx::KIND_MX && half && row < g.M && (col64 >> 5) < (int)g.y_across * mx::TILE_BLOCKS)
         *reinterpret_cast<uint16_t*>(g.ys + mx::scale_offset(row, col64 >> 5, g.y_across)) = (uint16_t)scales;
     if (!boxed) {
         if (row < g.M && col < g.N) store_direct<OUT>(g, row, col, w);
         return;
     }
-    if (BOX == 32 || first) {                              // the patch's last store has been read
-        if (lane == 0) tma_store_wait_read();
-        __syncwarp();
-    }
-    if (OUT == mx::KIND_MX) {
-        *reinterpret_cast<uint4*>(patch + lane * 32 + half * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
 #pragma unroll
-        for (int i = 0; i < WORDS / 4; ++i)                // 128-byte swizzle: 16-byte piece p of row r at p ^ (r & 7)
-            *reinterpret_cast<uint4*>(patch + lane * 128 + ((((BOX == 64 ? half * 4 : 0) + i) ^ (lane & 7)) << 4)) =
-                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    }
-    if (BOX == 32 || !first) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) tma_store_2d(map_y, patch, OUT == mx::KIND_MX ? col64 / 2 : BOX == 32 ? col : col64, (int)row0);
+    for (int q = 0; q < 32 / (BOX > 32 ? 32 : BOX); ++q) {
+        if (OUT != mx::KIND_MX || half == 0) {             // the patch's last store has been read
+            if (lane == 0) tma_store_wait_read();
+            __syncwarp();
+        }
+        if (OUT == mx::KIND_MX) {
+            *reinterpret_cast<uint4*>(patch + lane * 32 + half * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)                    // 64-byte swizzle: 16-byte piece p of row r at p ^ (r / 2 & 3)
+                *reinterpret_cast<uint4*>(patch + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(w[(16 * q + 4 * i) % WORDS], w[(16 * q + 4 * i + 1) % WORDS], w[(16 * q + 4 * i + 2) % WORDS], w[(16 * q + 4 * i + 3) % WORDS]);
+        }
+        if (OUT != mx::KIND_MX || half == 1) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma_store_2d(map_y, patch, OUT == mx::KIND_MX ? col64 / 2 : col + BOX * q, (int)row0);
+        }
     }
 }
 
@@ -218,7 +237,7 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* patches = smem + (size_t)STAGES * STAGE_BYTES;
-    Tail* tail = reinterpret_cast<Tail*>(patches + EPI_WARPS * PATCH_BYTES);
+    Tail* tail = reinterpret_cast<Tail*>(patches + EPI_WARPS * PATCH_BYTES + 2 * STASH_BYTES);
     constexpr int OUT_COLS = GATED ? 128 : 256;       // output features per tile
 
     const int warp = threadIdx.x >> 5;
@@ -232,8 +251,8 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         for (int s = 0; s < STAGES; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tail->tmem_full[a], 1);
-            mbar_init(&tail->tmem_empty[a], 2 * EPI_WARPS);
-            mbar_init(&tail->overlap_free[a], EPI_WARPS);      // one group of each CTA
+            mbar_init(&tail->tmem_empty[a], EPI_WARPS);         // two groups of each CTA
+            mbar_init(&tail->overlap_free[a], EPI_WARPS / 2);   // one
         }
         for (int i = 0; i < SF_SETS; ++i) mbar_init(&tail->sf_full[i], 1);
         tail->abort_flag = 0;
@@ -352,89 +371,81 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         __syncwarp();
     } else {
         const int quad = warp & 3;
-        const int grp = (warp - EPI_WARP0) >> 2;
-        const uint32_t lane_base = tmem_base + ((uint32_t)(quad * 32) << 16);
-        constexpr int HALF = 64;                               // columns per TMEM load step; the overlap lies within one
-        static_assert(OVERLAP <= HALF, "the overlap lies within one load step");
+        const int acc = (warp - EPI_WARP0) >> 3, half = ((warp - EPI_WARP0) >> 2) & 1;
+        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc ? ACC1 : 0);
         constexpr int COLS = GATED ? 64 : 128;                 // output columns per group
         uint8_t* patch = patches + (warp - EPI_WARP0) * PATCH_BYTES;
-        uint32_t scales = 0;
-        int it = 0;
-        bool ok = true;
-        auto release = [&](uint64_t* bar) {                    // this warp's part of an accumulator is in registers
+        // The columns that the accumulators share: the last of accumulator 0 (second half; gated: of the other factor), the first of
+        // accumulator 1 (first half; gated: of the gate).  Their group has them in `stash`, every thread its own row's.
+        const bool holder = half == 1 - acc;
+        const int shared0 = acc ? 0 : BN - OVERLAP;            // first shared column of the accumulator
+        float* stash = reinterpret_cast<float*>(patches + EPI_WARPS * PATCH_BYTES + acc * STASH_BYTES) + quad * 32 + lane;
+        static_assert(OVERLAP % 16 == 0 && OVERLAP <= COLS, "the shared columns are whole pieces of one group");
+        auto release = [&](uint64_t* bar) {                    // this warp has read its part
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mx::mbar_arrive_cluster(mx::map_to_cta(smem_u32(bar), 0));
         };
-        // Dense: all of a thread's 128 accumulator values go to registers before any is converted, the columns that the two
-        // accumulators share first, so the next tile's MMAs wait for the loads only and never for the arithmetic.
-        auto dense_tile = [&](int acc, long long row0, int n0) {
-            const uint32_t taddr = lane_base + (uint32_t)((acc ? ACC1 : 0) + grp * COLS);
-            const int up = acc ? 0 : 1;                        // the load step, and the group, that holds the shared columns
-            uint32_t r[4][32];                                 // pieces of 32 columns: of the first load step, then of the other
+        // 16 columns of the accumulator, from `c` on, of this thread's row
+        auto take = [&](int c, uint32_t* r) {
+            if (holder && (acc ? c < OVERLAP : c >= BN - OVERLAP)) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t at = taddr + (uint32_t)((i ^ up) * HALF);
-                tmem_ld32_async(at, r[2 * i]);
-                tmem_ld32_async(at + 32u, r[2 * i + 1]);
-                tmem_ld_wait32(r[2 * i]);
-                tmem_ld_wait32(r[2 * i + 1]);
-                if (i == 0 && grp == up) release(&tail->overlap_free[acc]);
-                if (i == 1) release(&tail->tmem_empty[acc]);
-            }
-            if (row0 >= g.M) return;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const int col = n0 + grp * COLS + ((p >> 1) ^ up) * HALF + 32 * (p & 1);
-                mx::f2 v[16];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = mx::pack2(__uint_as_float(r[p][2 * k]), __uint_as_float(r[p][2 * k + 1]));
-                if (g.bias[0]) add_bias(v, g.bias[0], col, g.N);
-                if (g.act == mx::ACT_RELU) mx::activate_pairs<16>(v, mx::ACT_RELU);
-                store32<OUT>(g, &map_y, patch, row0, lane, col, p & 1, (p & 1) == 0, scales, v);
+                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(stash[(c - shared0 + i) * 128]);
+            } else {
+                tmem_ld16_async(taddr + (uint32_t)c, r);
             }
         };
-        // Gated: 32 outputs at a time (64 registers of accumulators beside the activation's own); all at once as above spilled and
-        // ran 15 % slower on short reductions.  The shared columns are the second factor's last (accumulator 0) or the gate's
-        // first, so those pieces come first.
-        auto gated_tile = [&](int acc, long long row0, int n0) {
-            const uint32_t taddr = lane_base + (uint32_t)((acc ? ACC1 : 0) + grp * COLS);
-            const int up = acc == 0 && grp == 1;
-#pragma unroll 1
-            for (int j = 0; j < 2; ++j) {
-                const int half = j ^ up;
-                uint32_t a[32], u[32];
-                tmem_ld32_async(taddr + (uint32_t)(32 * half), a);
-                tmem_ld32_async(taddr + (uint32_t)(128 + 32 * half), u);
-                tmem_ld_wait32(a);
-                tmem_ld_wait32(u);
-                if (j == 1 && grp == 1 - acc) release(&tail->overlap_free[acc]);
-                if (j == 1) release(&tail->tmem_empty[acc]);
-                if (row0 >= g.M) continue;
-                const int col = n0 + grp * COLS + 32 * half;
-                mx::f2 v[16], w[16];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    v[k] = mx::pack2(__uint_as_float(a[2 * k]), __uint_as_float(a[2 * k + 1]));
-                    w[k] = mx::pack2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
-                }
-                if (g.bias[0]) add_bias(v, g.bias[0], col, g.N);
-                if (g.bias[1]) add_bias(w, g.bias[1], col, g.N);
-                mx::activate_pairs<16>(v, g.act);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = mx::mul2(v[k], w[k]);
-                store32<OUT>(g, &map_y, patch, row0, lane, col, half, j == 0, scales, v);
-            }
-        };
+        uint32_t scales = 0;
+        bool ok = true;
+        int it = 0;
         for (int tile = pair; tile < num_tiles; tile += num_pairs, ++it) {
+            if ((it & 1) != acc) continue;
             int mt, nt;
             tile_coords(tile, g, mt, nt);
             const long long row0 = (long long)mt * BM + (int)rank * BM_CTA + quad * 32;
-            if (ok) ok = mbar_wait(&tail->tmem_full[it & 1], (it >> 1) & 1, abort_flag, g.status, 165);
+            if (ok) ok = mbar_wait(&tail->tmem_full[acc], (it >> 1) & 1, abort_flag, g.status, 165);
             if (!ok) continue;
             tc_fence_after();
-            if (GATED) gated_tile(it & 1, row0, nt * OUT_COLS);
-            else dense_tile(it & 1, row0, nt * OUT_COLS);
+            if (holder) {
+                uint32_t r[OVERLAP];
+#pragma unroll
+                for (int i = 0; i < OVERLAP / 16; ++i) tmem_ld16_async(taddr + (uint32_t)(shared0 + 16 * i), r + 16 * i);
+#pragma unroll
+                for (int i = 0; i < OVERLAP / 16; ++i) tmem_ld_wait16(r + 16 * i);
+                release(&tail->overlap_free[acc]);
+#pragma unroll
+                for (int i = 0; i < OVERLAP; ++i) stash[i * 128] = __uint_as_float(r[i]);
+            }
+#pragma unroll 1
+            for (int p = 0; p < COLS / 32; ++p) {              // 32 outputs at a time
+                const int c = half * COLS + 32 * p, col = nt * OUT_COLS + c;
+                mx::f2 v[16];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t a[16], u[16];
+                    take(c + 16 * q, a);
+                    if (GATED) take(128 + c + 16 * q, u);
+                    tmem_ld_wait16(a);
+                    if (GATED) tmem_ld_wait16(u);
+                    if (q == 1 && p == COLS / 32 - 1) release(&tail->tmem_empty[acc]);
+                    mx::f2* x = v + 8 * q;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = mx::pack2(__uint_as_float(a[2 * k]), __uint_as_float(a[2 * k + 1]));
+                    if (g.bias[0]) add_bias(x, g.bias[0], col + 16 * q, g.N);
+                    if (GATED) {
+                        mx::f2 y[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) y[k] = mx::pack2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
+                        if (g.bias[1]) add_bias(y, g.bias[1], col + 16 * q, g.N);
+                        mx::activate_pairs<8>(x, g.act);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) x[k] = mx::mul2(x[k], y[k]);
+                    } else if (g.act == mx::ACT_RELU) {
+                        mx::activate_pairs<8>(x, mx::ACT_RELU);
+                    }
+                }
+                if (row0 < g.M) store32<OUT>(g, &map_y, patch, row0, lane, col, p & 1, scales, v);
+            }
         }
         if (lane == 0) tma_store_wait_read();      // the patch outlives its last store
     }

@@ -160,8 +160,10 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t local, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
     return a;
 }
+// Says that tensor memory has been read (tcgen05.wait::ld before it): no memory of this thread's is handed over, so the arrival
+// needs no release, which would first wait for the thread's stores.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
 }
 // TMA loads whose completion may be signalled on the peer CTA's barrier (cta_group::2 form, no multicast)
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
@@ -231,7 +233,7 @@ inline bool make_scale_map(CUtensorMap* map, const void* base, long long rows, i
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// an output [rows, cols] for TMA stores of 32 rows: 128 bytes of bf16 or f32 (128-byte swizzle), 32 bytes (64 codes) of MXFP4
+// an output [rows, cols] for TMA stores of 32 rows: 64 bytes of bf16 or f32 (64-byte swizzle), 32 bytes (64 codes) of MXFP4
 inline bool make_out_map(CUtensorMap* map, void* base, int kind, long long rows, int cols, long long ld) {
     const EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
@@ -239,11 +241,11 @@ inline bool make_out_map(CUtensorMap* map, void* base, int kind, long long rows,
     const int esz = kind == KIND_F32 ? 4 : 2;
     cuuint64_t dims[2] = {(cuuint64_t)(codes ? (cols + 1) / 2 : cols), (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)(codes ? ld / 2 : ld * esz)};
-    cuuint32_t box[2] = {(cuuint32_t)(codes ? 32 : 128 / esz), 32};
+    cuuint32_t box[2] = {(cuuint32_t)(codes ? 32 : 64 / esz), 32};
     cuuint32_t estr[2] = {1, 1};
     return fn(map, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : kind == KIND_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
               2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
