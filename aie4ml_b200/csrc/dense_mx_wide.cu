@@ -303,7 +303,7 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (leader && lane == 0) {
+        if (leader) {
             int stage = 0, it = 0, step = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -324,24 +324,28 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     const int steps = min(4, (g.K - kb * BK + 63) / 64);
                     const uint32_t sf = tmem_base + (uint32_t)(SF0 + (step % SF_SETS) * SF_COLS);
                     const uint64_t adesc = make_smem_desc(s), bdesc = make_smem_desc(s + CODE_BYTES);
+                    if (mx::elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (k >= steps) break;
-                        mx::umma_pair(d_tmem, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), g.idesc | mx::sf_bits(k & 1),
-                                      sf + (uint32_t)((k >> 1) * 4), sf + (uint32_t)(8 + (k >> 1) * 8), (uint32_t)((kb | k) != 0));
+                        for (int k = 0; k < 4; ++k) {
+                            if (k >= steps) break;
+                            mx::umma_pair(d_tmem, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), g.idesc | mx::sf_bits(k & 1),
+                                          sf + (uint32_t)((k >> 1) * 4), sf + (uint32_t)(8 + (k >> 1) * 8), (uint32_t)((kb | k) != 0));
+                        }
+                        mx::commit_pair(smem_u32(&tail->empty[stage]));
+                        mx::commit_pair(mx::map_to_cta(smem_u32(&tail->empty[stage]), 1));
+                        if (kb + 1 == g.num_kb) {
+                            mx::commit_pair(smem_u32(&tail->tmem_full[acc]));
+                            mx::commit_pair(mx::map_to_cta(smem_u32(&tail->tmem_full[acc]), 1));
+                        }
                     }
-                    mx::commit_pair(smem_u32(&tail->empty[stage]));
-                    mx::commit_pair(mx::map_to_cta(smem_u32(&tail->empty[stage]), 1));
+                    __syncwarp();
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
-                if (!ok) break;
-                mx::commit_pair(smem_u32(&tail->tmem_full[acc]));
-                mx::commit_pair(mx::map_to_cta(smem_u32(&tail->tmem_full[acc]), 1));
             }
         }
         __syncwarp();
     } else if (warp == 2) {
-        if (leader && lane == 0) {
+        if (leader) {
             const int total = ((num_tiles - pair + num_pairs - 1) / num_pairs) * g.num_kb;
             int stage = 0, kb = 0;
             uint32_t phase = 0;
@@ -354,16 +358,21 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 if (!ok) break;
                 tc_fence_after();
                 // columns of a set: A tile 0, A tile 1, weights tile 0 (8 columns: 256 rows), weights tile 1
-                const uint32_t f = smem_u32(smem) + (uint32_t)(stage * STAGE_BYTES + 2 * CODE_BYTES);
                 const uint32_t sf = tmem_base + (uint32_t)(SF0 + (step % SF_SETS) * SF_COLS);
-                const int halves = g.K - kb * BK > 128 ? 2 : 1;
-                for (int h = 0; h < halves; ++h) {
-                    const uint32_t t = (uint32_t)(h * mx::TILE_BYTES);
-                    mx::copy_scales_pair(sf + (uint32_t)(h * 4), mx::make_scale_desc(f + t));
-                    mx::copy_scales_pair(sf + (uint32_t)(8 + h * 8), mx::make_scale_desc(f + SF_BYTES + t));
-                    mx::copy_scales_pair(sf + (uint32_t)(12 + h * 8), mx::make_scale_desc(f + 2 * SF_BYTES + t));
+                const uint64_t f = mx::make_scale_desc(smem_u32(smem) + (uint32_t)(stage * STAGE_BYTES + 2 * CODE_BYTES));
+                const bool both = g.K - kb * BK > 128;
+                if (mx::elect_one()) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h == 1 && !both) break;
+                        const uint64_t t = f + (uint64_t)(h * (mx::TILE_BYTES >> 4));
+                        mx::copy_scales_pair(sf + (uint32_t)(h * 4), t);
+                        mx::copy_scales_pair(sf + (uint32_t)(8 + h * 8), t + (uint64_t)(SF_BYTES >> 4));
+                        mx::copy_scales_pair(sf + (uint32_t)(12 + h * 8), t + (uint64_t)(2 * SF_BYTES >> 4));
+                    }
+                    mx::commit_pair(smem_u32(&tail->sf_full[step % SF_SETS]));
                 }
-                mx::commit_pair(smem_u32(&tail->sf_full[step % SF_SETS]));
+                __syncwarp();
                 if (++kb == g.num_kb) kb = 0;
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }

@@ -102,6 +102,15 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t adesc, uint64_t b
         :: "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
 }
 
+// true in one lane of a converged warp.  The tensor-core roles run their loops with whole warps and elect a lane for the
+// instructions themselves: descriptors then stay in uniform registers, where a loop inside `if (lane == 0)` moves each of
+// them over for every instruction.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // A 512-byte scale tile as the source of tcgen05.cp: 32 rows of 16 bytes without swizzle, 8-row groups 128 bytes apart.
 __device__ __forceinline__ uint64_t make_scale_desc(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
