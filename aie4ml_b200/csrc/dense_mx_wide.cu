@@ -331,12 +331,8 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                             mx::umma_pair(d_tmem, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), g.idesc | mx::sf_bits(k & 1),
                                           sf + (uint32_t)((k >> 1) * 4), sf + (uint32_t)(8 + (k >> 1) * 8), (uint32_t)((kb | k) != 0));
                         }
-                        mx::commit_pair(smem_u32(&tail->empty[stage]));
-                        mx::commit_pair(mx::map_to_cta(smem_u32(&tail->empty[stage]), 1));
-                        if (kb + 1 == g.num_kb) {
-                            mx::commit_pair(smem_u32(&tail->tmem_full[acc]));
-                            mx::commit_pair(mx::map_to_cta(smem_u32(&tail->tmem_full[acc]), 1));
-                        }
+                        mx::commit_both(smem_u32(&tail->empty[stage]));
+                        if (kb + 1 == g.num_kb) mx::commit_both(smem_u32(&tail->tmem_full[acc]));
                     }
                     __syncwarp();
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
