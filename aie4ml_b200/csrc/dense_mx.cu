@@ -14,9 +14,9 @@
 // rank sends its partial sums to the rank that finishes the row (distributed shared memory), which adds them in rank order,
 // so the result does not depend on timing and no workspace exists.
 //
-// One tile per CTA: warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue, of which warp 2 first moves the scales on to
-// TMEM (tcgen05.cp; a set of columns per stage, so it runs ahead of the MMAs; copies issued by the MMA thread run in turn with
-// its MMAs and held a stage at 0.6 us).  A stage is 256 values of K: 128-byte swizzled rows of codes and the scale tiles.
+// One tile per CTA: warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue.  A stage is 256 values of K: 128-byte swizzled
+// rows of codes and the scale tiles, which the issuer copies on to TMEM (tcgen05.cp) ahead of the stage's MMAs; the tensor pipe
+// takes both in issue order.
 // A CTA runs all of its code once, so unrolled code costs its way out of memory: the epilogue converts 16 rows at a time.
 // Every wait is bounded.
 #include <cuda.h>
@@ -45,7 +45,7 @@ constexpr size_t ONE_PER_SM = 116 * 1024;
 struct Tail {
     uint64_t full[MAX_STAGES];
     uint64_t empty[MAX_STAGES];
-    uint64_t scaled[MAX_STAGES];     // the stage's scales lie in tensor memory
+    uint64_t moved[MAX_STAGES];      // the stage's A scales lie in the first column
     uint64_t done;
     uint32_t tmem_base;
     volatile int abort_flag;
@@ -177,7 +177,7 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     };
     const int ahead = min(g.stages, kb1 - kb0);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < g.stages; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); mbar_init(&tail->scaled[s], 1); }
+        for (int s = 0; s < g.stages; ++s) { mbar_init(&tail->full[s], 1); mbar_init(&tail->empty[s], 1); mbar_init(&tail->moved[s], 1); }
         mbar_init(&tail->done, 1);
         tail->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -210,59 +210,56 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                ok = mbar_wait(&tail->scaled[stage], phase, abort_flag, g.status, 152) &&
-                     mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 154);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t s = smem_u32(smem) + (uint32_t)(stage * g.stage_bytes);
-                const int steps = min(4, (g.K - kb * BK + 63) / 64);   // MMAs of 64 values; beyond K nothing is read
-                const uint32_t sf = tmem_base + (uint32_t)(SF0 + stage * SF_COLS);
-                const uint64_t wdesc = make_smem_desc(s), adesc = make_smem_desc(s + NW * W_BYTES);
-#pragma unroll 1
-                for (int k = 0; k < steps; ++k) {
-                    const uint32_t idesc = g.idesc | mx::sf_bits(k & 1);
-#pragma unroll
-                    for (int o = 0; o < NW; ++o)
-                        mx::umma(tmem_base + (uint32_t)(o * MAX_T), wdesc + (uint64_t)(o * (W_BYTES >> 4) + k * 2), adesc + (uint64_t)(k * 2), idesc,
-                                 sf + (uint32_t)(o * 8 + (k >> 1) * 4), sf + (uint32_t)(NW * 8 + (k >> 1) * 4), (uint32_t)(kb != kb0 || k != 0));
-                }
-                umma_commit(&tail->empty[stage]);
-                if (++stage == g.stages) { stage = 0; phase ^= 1u; }
-            }
-            if (ok) umma_commit(&tail->done);
-        }
-        __syncwarp();
-    } else if (warp == 2) {
-        // a stage's columns were last read by the MMAs whose completion let the stage be filled again
         int stage = 0;
         uint32_t phase = 0;
+        bool ok = true;
         for (int kb = kb0; kb < kb1; ++kb) {
-            if (!mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 155)) break;
-            uint8_t* f = smem + (size_t)(stage + 1) * g.stage_bytes - (NW + 1) * SF_BYTES;
-            const int halves = min(2, g.k_tiles - 2 * kb);             // scale tiles of 128 values of K
-            if (sf_row != 0) {
-                uint32_t* fa = reinterpret_cast<uint32_t*>(f + NW * SF_BYTES) + lane * 4;
-                for (int h = 0; h < halves; ++h) fa[h * (mx::TILE_BYTES / 4)] = fa[h * (mx::TILE_BYTES / 4) + sf_row];
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-            }
-            if (lane == 0) {
-                tc_fence_after();
-                const uint32_t sf = tmem_base + (uint32_t)(SF0 + stage * SF_COLS);
+            ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 152) &&
+                 (sf_row == 0 || mbar_wait(&tail->moved[stage], phase, abort_flag, g.status, 154));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t s = smem_u32(smem) + (uint32_t)(stage * g.stage_bytes);
+            const int steps = min(4, (g.K - kb * BK + 63) / 64);   // MMAs of 64 values; beyond K nothing is read
+            const uint32_t sf = tmem_base + (uint32_t)(SF0 + stage * SF_COLS);
+            const uint64_t wdesc = make_smem_desc(s), adesc = make_smem_desc(s + NW * W_BYTES);
+            const uint64_t fdesc = mx::make_scale_desc(s + (uint32_t)(g.stage_bytes - (NW + 1) * SF_BYTES));
+            if (mx::elect_one()) {
 #pragma unroll
-                for (int o = 0; o < NW + 1; ++o)
-                    for (int h = 0; h < halves; ++h)
-                        mx::copy_scales(sf + (uint32_t)(o * 8 + h * 4), mx::make_scale_desc(smem_u32(f) + (uint32_t)(o * SF_BYTES + h * mx::TILE_BYTES)));
-                umma_commit(&tail->scaled[stage]);
+                for (int h = 0; h < 2; ++h) {                      // scale tiles of 128 values of K
+                    if (steps <= 2 * h) break;
+#pragma unroll
+                    for (int o = 0; o < NW + 1; ++o)
+                        mx::copy_scales(sf + (uint32_t)(o * 8 + h * 4), fdesc + (uint64_t)((o * SF_BYTES + h * mx::TILE_BYTES) >> 4));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (k >= steps) break;
+#pragma unroll
+                    for (int o = 0; o < NW; ++o)
+                        mx::umma(tmem_base + (uint32_t)(o * MAX_T), wdesc + (uint64_t)(o * (W_BYTES >> 4) + k * 2), adesc + (uint64_t)(k * 2),
+                                 g.idesc | mx::sf_bits(k & 1), sf + (uint32_t)(o * 8 + (k >> 1) * 4), sf + (uint32_t)(NW * 8 + (k >> 1) * 4),
+                                 (uint32_t)(kb != kb0 || k != 0));
+                }
+                umma_commit(&tail->empty[stage]);
+                if (kb + 1 == kb1) umma_commit(&tail->done);
             }
             __syncwarp();
             if (++stage == g.stages) { stage = 0; phase ^= 1u; }
         }
+    } else if (warp == 2 && sf_row != 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 155)) break;
+            uint32_t* f = reinterpret_cast<uint32_t*>(smem + (size_t)(stage + 1) * g.stage_bytes - SF_BYTES) + lane * 4;
+            f[0] = f[sf_row];
+            if (g.k_tiles - 2 * kb > 1) f[mx::TILE_BYTES / 4] = f[mx::TILE_BYTES / 4 + sf_row];
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tail->moved[stage]);
+            if (++stage == g.stages) { stage = 0; phase ^= 1u; }
+        }
+        __syncwarp();
     }
 
     const int quad = warp & 3;

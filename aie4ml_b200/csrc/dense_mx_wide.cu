@@ -13,11 +13,12 @@
 // accumulators overlap by 48 columns.  The epilogue first moves those to shared memory and says so on a barrier of its own;
 // the next tile's MMAs wait for that and not for the tile's arithmetic.
 //
-// The scale copies (tcgen05.cp) have a warp of their own, one stage ahead of the MMAs and tied to them by barriers: issued
-// by the MMA thread they run in turn with the MMAs, six copies of a stage costing 0.22 us on top of its 0.40 us of MMAs
-// (4096 x 16384 x 8192: 303 us; spread out between the MMAs 346 us; from their own warp 240 us, no copies at all 205 us).
+// The scale copies (tcgen05.cp) go down the tensor pipe with the MMAs, which takes both in issue order, so they need no barrier
+// when one thread issues both (from a warp of their own, with barriers, a stage took 806 cycles; from here 670).  That thread is
+// an elected lane of a converged warp: in a loop under `if (lane == 0)` every descriptor is first moved to a uniform register,
+// and the MMAs of a stage took 940 cycles to issue, longer than the 512 they run.
 //
-// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2 scale copies (leader CTA), 3-18 epilogue: two groups of four warps per
+// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-17 epilogue: two groups of four warps per
 // accumulator, each half of the columns, so that two tiles are converted at once.  A lane holds one row, so an MXFP4 output block
 // is 32 values of one thread; rows go out through a swizzled patch of shared memory per warp and TMA stores (directly from
 // registers every 16 bytes of a row were an L2 request of their own).  Every wait is bounded.
@@ -45,7 +46,7 @@ constexpr int SF0 = TMEM_COLS - SF_SETS * SF_COLS;
 constexpr int ACC1 = SF0 - BN;                // second accumulator: columns ACC1 .. SF0
 constexpr int OVERLAP = BN - ACC1;
 constexpr int EPI_WARPS = 16;
-constexpr int EPI_WARP0 = 3;                   // first epilogue warp
+constexpr int EPI_WARP0 = 2;                   // first epilogue warp
 constexpr int NUM_THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
 constexpr int PATCH_BYTES = 32 * 64;            // per epilogue warp: 32 rows of a TMA store's box
 constexpr int STASH_BYTES = OVERLAP * 128 * 4;  // per accumulator: the shared columns of this CTA's rows, [column][row]
@@ -56,7 +57,6 @@ struct Tail {
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
     uint64_t overlap_free[2];
-    uint64_t sf_full[SF_SETS];
     uint32_t tmem_base;
     volatile int abort_flag;
 };
@@ -254,7 +254,6 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             mbar_init(&tail->tmem_empty[a], EPI_WARPS);         // two groups of each CTA
             mbar_init(&tail->overlap_free[a], EPI_WARPS / 2);   // one
         }
-        for (int i = 0; i < SF_SETS; ++i) mbar_init(&tail->sf_full[i], 1);
         tail->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -316,15 +315,24 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(acc ? ACC1 : 0);
                 for (int kb = 0; kb < g.num_kb; ++kb, ++step) {
-                    ok = mbar_wait(&tail->sf_full[step % SF_SETS], (step / SF_SETS) & 1, abort_flag, g.status, 164) &&
-                         mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 164);
+                    ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 164);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t s = smem_u32(smem) + (uint32_t)(stage * STAGE_BYTES);
                     const int steps = min(4, (g.K - kb * BK + 63) / 64);
                     const uint32_t sf = tmem_base + (uint32_t)(SF0 + (step % SF_SETS) * SF_COLS);
                     const uint64_t adesc = make_smem_desc(s), bdesc = make_smem_desc(s + CODE_BYTES);
+                    // columns of a set: A tile 0, A tile 1, weights tile 0 (8 columns: 256 rows), weights tile 1
+                    const uint64_t fdesc = mx::make_scale_desc(s + 2 * CODE_BYTES);
                     if (mx::elect_one()) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (steps <= 2 * h) break;
+                            const uint64_t t = fdesc + (uint64_t)(h * (mx::TILE_BYTES >> 4));
+                            mx::copy_scales_pair(sf + (uint32_t)(h * 4), t);
+                            mx::copy_scales_pair(sf + (uint32_t)(8 + h * 8), t + (uint64_t)(SF_BYTES >> 4));
+                            mx::copy_scales_pair(sf + (uint32_t)(12 + h * 8), t + (uint64_t)(2 * SF_BYTES >> 4));
+                        }
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             if (k >= steps) break;
@@ -337,40 +345,6 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     __syncwarp();
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
-            }
-        }
-        __syncwarp();
-    } else if (warp == 2) {
-        if (leader) {
-            const int total = ((num_tiles - pair + num_pairs - 1) / num_pairs) * g.num_kb;
-            int stage = 0, kb = 0;
-            uint32_t phase = 0;
-            for (int step = 0; step < total; ++step) {
-                bool ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 166);
-                if (ok && step >= SF_SETS) {           // the MMAs that read this set's last contents are done
-                    const int old = step - SF_SETS;
-                    ok = mbar_wait(&tail->empty[old % STAGES], (old / STAGES) & 1, abort_flag, g.status, 167);
-                }
-                if (!ok) break;
-                tc_fence_after();
-                // columns of a set: A tile 0, A tile 1, weights tile 0 (8 columns: 256 rows), weights tile 1
-                const uint32_t sf = tmem_base + (uint32_t)(SF0 + (step % SF_SETS) * SF_COLS);
-                const uint64_t f = mx::make_scale_desc(smem_u32(smem) + (uint32_t)(stage * STAGE_BYTES + 2 * CODE_BYTES));
-                const bool both = g.K - kb * BK > 128;
-                if (mx::elect_one()) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h == 1 && !both) break;
-                        const uint64_t t = f + (uint64_t)(h * (mx::TILE_BYTES >> 4));
-                        mx::copy_scales_pair(sf + (uint32_t)(h * 4), t);
-                        mx::copy_scales_pair(sf + (uint32_t)(8 + h * 8), t + (uint64_t)(SF_BYTES >> 4));
-                        mx::copy_scales_pair(sf + (uint32_t)(12 + h * 8), t + (uint64_t)(2 * SF_BYTES >> 4));
-                    }
-                    mx::commit_pair(smem_u32(&tail->sf_full[step % SF_SETS]));
-                }
-                __syncwarp();
-                if (++kb == g.num_kb) kb = 0;
-                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
         }
         __syncwarp();
