@@ -8,7 +8,7 @@ C ABI in ``include/aie4ml_b200.h``.
 
 from .frontends.graph import GraphBuilder, intent, lower_graph_dict
 from .model import CudaModel, from_graph
-from .qtypes import AIEDataType, QuantIntent, RoundingMode, SaturationMode
+from .qtypes import MXFP4, AIEDataType, FloatFormat, FloatIntent, QuantIntent, RoundingMode, SaturationMode
 
 __version__ = '0.1.0'
 
@@ -21,5 +21,5 @@ def from_onnx(model_or_path, config, *, output_dir=None, project_name=None, **kw
     return _from_onnx(model_or_path, config, output_dir=output_dir, project_name=project_name, **kwargs)
 
 
-__all__ = ['AIEDataType', 'CudaModel', 'GraphBuilder', 'QuantIntent', 'RoundingMode', 'SaturationMode', 'from_graph',
+__all__ = ['AIEDataType', 'CudaModel', 'FloatFormat', 'FloatIntent', 'GraphBuilder', 'MXFP4', 'QuantIntent', 'RoundingMode', 'SaturationMode', 'from_graph',
            'from_onnx', 'intent', 'lower_graph_dict']

@@ -18,7 +18,7 @@ from typing import Any, Dict, List, Optional, Sequence, Tuple
 import numpy as np
 
 from ..ir import BackendContext, DEVICE_CATALOG, LogicalIR, OpNode, TensorVar, set_input_roles
-from ..qtypes import QuantIntent, RoundingMode, SaturationMode
+from ..qtypes import _FORMATS, MXFP4, FloatFormat, FloatIntent, QuantIntent, RoundingMode, SaturationMode
 
 _KNOWN_DIRECTIVES = ('placement', 'microtiling', 'parallelism', 'io_route', 'layout', 'approximation', 'hccs')
 
@@ -134,13 +134,23 @@ class GraphBuilder:
     def dense(self, name: str, x: str, weight, w_precision: QuantIntent, out_precision: QuantIntent, *,
               bias=None, bias_precision: Optional[QuantIntent] = None, relu: bool = False,
               relu_precision: Optional[QuantIntent] = None, out_name: Optional[str] = None) -> str:
-        """``y = relu?(x @ W + b)``; W is ``[K, N]`` float (code / 2**frac)."""
+        """``y = relu?(x @ W + b)``; W is ``[K, N]`` float (code / 2**frac), or held in MXFP4 when ``w_precision`` is
+        ``qtypes.MXFP4`` (the input then is bfloat16 or float32, and the bias float32 without a precision)."""
         W = np.asarray(weight, dtype=np.float64)
         xs = self._t(x).shape
         if W.ndim != 2 or int(xs[-1]) != W.shape[0]:
             raise ValueError(f'{name}: weight shape {W.shape} does not match input features {xs[-1]}.')
         out_shape = tuple(xs[:-1]) + (W.shape[1],)
         final = out_name or f'{name}_out'
+        if w_precision == MXFP4:     # one node: bias and ReLU are the product's own
+            ins = [x, self.param(f'{name}_weight', W, w_precision)]
+            if bias is not None:
+                ins.append(self.param(f'{name}_biasv', np.asarray(bias, dtype=np.float64).reshape(-1), None))
+            self.emit('mx_dense', name, ins, [(final, out_shape, (relu_precision if relu else None) or out_precision)],
+                      roles=['lhs', 'rhs', 'bias'][:len(ins)],
+                      metadata={'n_in': int(W.shape[0]), 'n_out': int(W.shape[1]), 'activation': 'relu' if relu else 'none',
+                                'layer_class': 'Dense', 'source_layer': name})
+            return final
         stages = ['mm'] + (['bias'] if bias is not None else []) + (['relu'] if relu else [])
         names = [f'{name}_{s}' for s in stages[:-1]] + [final]
         self.param(f'{name}_weight', W, w_precision)
@@ -163,6 +173,26 @@ class GraphBuilder:
                       [(names[cur + 1], out_shape, relu_precision or out_precision)], roles=['lhs'],
                       metadata={'activation': 'relu', 'layer_class': 'Activation', 'source_layer': name})
         return final
+
+    def gated_dense(self, name: str, x: str, w_gate, w_up, w_precision, out_precision, *, activation: str = 'silu', bias_gate=None,
+                    bias_up=None, out_name: Optional[str] = None) -> str:
+        """``y = activation(x @ Wg + bg) * (x @ Wu + bu)``, the first half of a gated feed-forward block; both weights are
+        ``[K, N]`` float, held as ``w_precision`` (``qtypes.MXFP4``)."""
+        xs = self._t(x).shape
+        shapes = [np.asarray(w).shape for w in (w_gate, w_up)]
+        if len(shapes[0]) != 2 or shapes[0] != shapes[1] or int(xs[-1]) != shapes[0][0]:
+            raise ValueError(f'{name}: weight shapes {shapes} do not match input features {xs[-1]}.')
+        ins, roles = [x], ['lhs']
+        for role, data, precision in (('gate', w_gate, w_precision), ('up', w_up, w_precision), ('gate_bias', bias_gate, None),
+                                      ('up_bias', bias_up, None)):
+            if data is not None:
+                ins.append(self.param(f'{name}_{role}', data, precision))
+                roles.append(role)
+        out = out_name or f'{name}_out'
+        self.emit('gated_dense', name, ins, [(out, tuple(xs[:-1]) + (shapes[0][1],), out_precision)], roles=roles,
+                  metadata={'n_in': int(shapes[0][0]), 'n_out': int(shapes[0][1]), 'activation': str(activation),
+                            'layer_class': 'GatedDense', 'source_layer': name})
+        return out
 
     def matmul(self, name: str, a: str, b: str, out_precision: QuantIntent, out_name: Optional[str] = None) -> str:
         sa, sb = self._t(a).shape, self._t(b).shape
@@ -288,8 +318,11 @@ class GraphBuilder:
 def _prec(d) -> Optional[QuantIntent]:
     if d is None:
         return None
-    if isinstance(d, QuantIntent):
+    if isinstance(d, (QuantIntent, FloatIntent)):
         return d
+    if 'float' in d:
+        fmt = FloatFormat(str(d['float']))
+        return FloatIntent(width=_FORMATS[fmt.value][0], format=fmt)
     return QuantIntent.from_dict(d)
 
 
@@ -298,7 +331,8 @@ def lower_graph_dict(spec: Dict[str, Any], config: Optional[Dict[str, Any]] = No
 
     Each node is ``{'name', 'op', 'inputs': [tensor names], 'outputs': [{'name','shape','precision'}],
     'roles': [...], 'metadata': {...}}`` with ``op`` one of dense, matmul, add, activation, scale,
-    softmax, layer_norm, transpose, slice, split, concat -- the op vocabulary of the logical IR."""
+    mx_dense, gated_dense, softmax, layer_norm, transpose, slice, split, concat -- the op vocabulary of the logical IR.  A precision
+    ``{'float': 'mxfp4'}`` (or another float format) is a floating-point one."""
     b = GraphBuilder(config, name=str(spec.get('name', 'model')))
     for item in spec.get('inputs', []):
         b.input(item['name'], item['shape'], _prec(item['precision']))

@@ -72,6 +72,7 @@ class CudaModel:
                              merge_parallel_dense=bool(fusion.get('parallel_dense', True)),
                              fuse_dense_chain=bool(fusion.get('dense_chain', True)),
                              fuse_dense_ln=bool(fusion.get('dense_ln', True)),
+                             fuse_mx_chain=bool(fusion.get('mx_chain', True)),
                              dense_algo=int(self._ctx.aie_config.get('DenseAlgo', 0)))
         return 0
 

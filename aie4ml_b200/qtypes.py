@@ -58,6 +58,7 @@ class FloatFormat(Enum):
     BF16 = 'bfloat16'
     FP32 = 'float32'
     FP8_E4M3 = 'fp8_e4m3'
+    MXFP4 = 'mxfp4'
 
 
 @dataclass(frozen=True)
@@ -71,11 +72,16 @@ class FloatIntent:
 
 FLOAT_FORMATS = ('bfloat16', 'float32', 'fp8_e4m3')
 
+# Weights held in blocks of 32 four-bit values with a power-of-two scale each: the ``w_precision`` that selects the MXFP4
+# products (an activation tensor is never stored this way by name; the plan quantises it where such a product reads it).
+MXFP4 = FloatIntent(width=4, format=FloatFormat.MXFP4)
+
 # format -> (bits, signed, numpy dtype, C type); bfloat16 is stored as its 16 bits, fp8 (E4M3, finite-only) as its 8
 _FORMATS = {
     'bfloat16': (16, True, np.uint16, 'uint16_t'),
     'float32': (32, True, np.float32, 'float'),
     'fp8_e4m3': (8, True, np.uint8, 'uint8_t'),
+    'mxfp4': (4, True, np.uint8, 'uint8_t'),
     'int8': (8, True, np.int8, 'int8_t'),
     'uint8': (8, False, np.uint8, 'uint8_t'),
     'int16': (16, True, np.int16, 'int16_t'),

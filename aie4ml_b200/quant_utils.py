@@ -169,3 +169,55 @@ def from_storage_float(stored, fmt: str) -> np.ndarray:
     if fmt == 'fp8_e4m3':
         return from_fp8_bits(stored)
     return np.asarray(stored, dtype=np.float32)
+
+
+# ---- MXFP4: blocks of 32 four-bit values (E2M1) along a row, a power-of-two scale (E8M0) each --------------------------------
+_E2M1 = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def mx_pitch(cols: int) -> int:
+    """Row pitch of the codes in elements: whole 16-byte pieces."""
+    return (int(cols) + 31) // 32 * 32
+
+
+def to_mx(values):
+    """float ``[rows, cols]`` -> (codes uint8 ``[rows, pitch / 2]``, scale tiles uint8), as ``a4c_quantize_mx`` lays them out
+    (include/aie4ml_b200.h): scale 2^max(floor(log2 max|x|) - 2, -127), codes to nearest even, saturating at 6."""
+    x = np.asarray(values, dtype=np.float64)
+    if x.ndim != 2 or x.shape[0] < 1 or x.shape[1] < 1:
+        raise ValueError(f'to_mx: expected a matrix, got shape {x.shape}.')
+    rows, cols = x.shape
+    pitch = mx_pitch(cols)
+    blocks = pitch // 32
+    v = np.zeros((rows, pitch))
+    v[:, :cols] = x
+    v = v.reshape(rows, blocks, 32)
+    bad = ~np.isfinite(v).all(axis=2)
+    v = np.where(bad[:, :, None], 0.0, v)
+    top = np.abs(v).max(axis=2)
+    exponent = np.where(top > 0, np.frexp(top)[1] - 3, -127)          # frexp: top = m 2^e with 0.5 <= m < 1
+    exponent = np.maximum(exponent, -127)
+    a = np.ldexp(np.abs(v), -exponent[:, :, None])
+    # the borders between neighbouring magnitudes; on 0.25, 1.25, 2.5 and 5 the lower (even) code stays
+    mids = (_E2M1[1:] + _E2M1[:-1]) / 2
+    code = np.zeros(a.shape, dtype=np.uint8)
+    for i, mid in enumerate(mids):
+        code += (a >= mid) if i % 2 else (a > mid)
+    code |= np.signbit(v).astype(np.uint8) << 3
+    code = code.reshape(rows, pitch)
+    code[:, cols:] = 0
+    scales = np.zeros(((rows + 127) // 128 * 128, (blocks + 3) // 4 * 4), dtype=np.uint8)
+    scales[:rows, :blocks] = np.where(bad, 255, exponent + 127)
+    tiles = scales.reshape(-1, 4, 32, scales.shape[1] // 4, 4).transpose(0, 3, 2, 1, 4)
+    return code[:, 0::2] | (code[:, 1::2] << 4), np.ascontiguousarray(tiles).reshape(-1)
+
+
+def from_mx(codes, tiles, rows: int, cols: int) -> np.ndarray:
+    """The float32 values that codes and scale tiles stand for."""
+    codes = np.asarray(codes, dtype=np.uint8)
+    c = np.stack([codes & 15, codes >> 4], axis=2).reshape(rows, -1)[:, :cols]
+    across = (cols + 127) // 128
+    s = np.asarray(tiles).reshape(-1, across, 32, 4, 4).transpose(0, 3, 2, 1, 4).reshape(-1, across * 4)[:rows]
+    scale = np.where(s == 255, np.nan, np.ldexp(1.0, s.astype(np.int32) - 127))
+    mag = np.where(c & 8, -_E2M1[c & 7], _E2M1[c & 7])
+    return (mag * np.repeat(scale, 32, axis=1)[:, :cols]).astype(np.float32)

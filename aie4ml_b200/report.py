@@ -63,6 +63,15 @@ def op_cost(plan, op: Dict[str, Any]) -> Dict[str, float]:
         nq, nk = heads * _numel(plan, op['q']), heads * _numel(plan, op['k'])
         sk, dh = k.shape[-2], k.shape[-1]
         return {'bytes': 2 * nq + 2 * nk, 'ops': 2.0 * (nq // dh) * sk * dh * 2}
+    if kind == 'quantize_mx':
+        n = _numel(plan, op['lhs'])
+        return {'bytes': n * plan.views[op['lhs']].esz + sum(t.numel() for t in plan.mx[op['lhs']]), 'ops': 0.0}
+    if kind in ('dense_mx', 'gated_dense_mx'):
+        M, weights = int(plan.mx[op['lhs']][0].shape[0]), ('weight',) if kind == 'dense_mx' else ('gate', 'up')
+        mx = lambda rows, cols: rows * ((cols + 1) // 2 + (cols + 31) // 32)
+        out = mx(M, op['N']) if op.get('out_mx') else M * op['N'] * plan.views[op['out']].esz
+        return {'bytes': mx(M, op['K']) + len(weights) * mx(op['N'], op['K']) + out,
+                'ops': 2.0 * M * op['K'] * op['N'] * len(weights)}
     if kind in ('layer_norm', 'softmax', 'add'):
         n = _numel(plan, op['lhs'])
         b = n * esz(op['lhs']) + _numel(plan, op['out']) * esz(op['out'])

@@ -20,7 +20,8 @@ import numpy as np
 
 from . import lib as _lib
 from .ir import BackendContext, input_tensor_for_role
-from .op_impls.precision import DTYPE_CODE, FLOAT_CODE, ROUNDING_CODE, resolve_exact_storage_dtype
+from .op_impls.precision import ACTIVATION_CODE, DTYPE_CODE, FLOAT_CODE, ROUNDING_CODE, resolve_exact_storage_dtype
+from .quant_utils import mx_pitch
 
 ESZ = {'int8': 1, 'uint8': 1, 'int16': 2, 'int32': 4, 'bfloat16': 2, 'float32': 4, 'fp8_e4m3': 1}
 NP_DT = {'int8': np.int8, 'uint8': np.uint8, 'int16': np.int16, 'int32': np.int32, 'bfloat16': np.uint16,
@@ -112,7 +113,7 @@ class Plan:
     def __init__(self, ctx: BackendContext, device: Optional[str] = None, fuse_rowop_add: bool = True,
                  dense_algo: int = _lib.ALGO_AUTO, share_params: Optional['Plan'] = None, fuse_attention: bool = True,
                  fuse_dense_chain: bool = True, merge_attention_heads: bool = True, merge_parallel_dense: bool = True,
-                 fuse_dense_ln: bool = True):
+                 fuse_dense_ln: bool = True, fuse_mx_chain: bool = True):
         torch = _torch()
         self.ctx = ctx
         self.lib = _lib.load()
@@ -124,10 +125,10 @@ class Plan:
         # entry into it from this plan runs with the plan's device current, whatever the caller had selected.
         with torch.cuda.device(self.device):
             self._build(ctx, fuse_rowop_add, dense_algo, share_params, fuse_attention, fuse_dense_chain,
-                        merge_attention_heads, merge_parallel_dense, fuse_dense_ln)
+                        merge_attention_heads, merge_parallel_dense, fuse_dense_ln, fuse_mx_chain)
 
     def _build(self, ctx, fuse_rowop_add, dense_algo, share_params, fuse_attention, fuse_dense_chain,
-               merge_attention_heads, merge_parallel_dense, fuse_dense_ln) -> None:
+               merge_attention_heads, merge_parallel_dense, fuse_dense_ln, fuse_mx_chain) -> None:
         torch = _torch()
         self.dense_algo = int(dense_algo)
         self.fuse_rowop_add = bool(fuse_rowop_add)
@@ -177,6 +178,13 @@ class Plan:
                 self.params_np[op['weight']] = inst.artifacts['packed_weights']
                 if op['bias']:
                     self.params_np[op['bias']] = inst.artifacts['packed_bias']
+            elif op['kind'] == 'dense_mx':
+                self._mx_params(op, 'weight', 'bias', inst.artifacts['packed_weights'], inst.artifacts['packed_scales'],
+                                inst.artifacts['packed_bias'])
+            elif op['kind'] == 'gated_dense_mx':
+                for role in ('gate', 'up'):
+                    self._mx_params(op, role, f'{role}_bias', inst.artifacts[f'packed_{role}'],
+                                    inst.artifacts[f'packed_{role}_scales'], inst.artifacts[f'packed_{role}_bias'])
             elif op['kind'] == 'layer_norm':
                 self.params_np[op['gamma']] = inst.artifacts['packed_gamma']
                 self.params_np[op['beta']] = inst.artifacts['packed_beta']
@@ -189,6 +197,7 @@ class Plan:
         self.views: Dict[str, View] = {}
         self.buffers: Dict[str, Any] = {}
         self.synthetic: Dict[str, Tuple[int, ...]] = {}     # tensors the plan adds (name -> shape): merged outputs
+        self.mx: Dict[str, Tuple[Any, Any]] = {}            # MXFP4 form of an activation: (codes, scale tiles)
         if merge_parallel_dense:
             self._merge_parallel_dense()
         if fuse_attention:
@@ -203,11 +212,13 @@ class Plan:
             if fuse_dense_ln:
                 self._fuse_dense_add_layernorm()
             self._fuse_rowop_add()
+        self.fuse_mx_chain = bool(fuse_mx_chain)
+        self._quantize_mx_inputs()
 
         live = set(graph.input_tensor_names) | set(graph.output_tensor_names)
         for op in self.ops:
             for key in ('lhs', 'rhs', 'out', 'addend', 'pre_addend', 'residual', 'q', 'k', 'v'):
-                if op.get(key):
+                if op.get(key) and not self._only_mx(op, key):
                     live.add(op[key])
             for member in op.get('members', ()):
                 live.update(member.values())
@@ -354,6 +365,67 @@ class Plan:
             self.fused.append(merged_name)
         if replace:
             self.ops = [replace.get(i, op) for i, op in enumerate(self.ops) if i not in drop]
+
+    def _mx_params(self, op, weight, bias, codes, tiles, bias_values) -> None:
+        self.params_np[op[weight]] = codes
+        self.params_np[op[weight] + '.scales'] = tiles
+        if op[bias]:
+            self.params_np[op[bias]] = bias_values
+
+    @staticmethod
+    def _only_mx(op: Dict[str, Any], key: str) -> bool:
+        """The op touches this tensor in its MXFP4 form alone (no float buffer is needed for it)."""
+        return (key == 'lhs' and op['kind'] in ('dense_mx', 'gated_dense_mx')) or (key == 'out' and bool(op.get('out_mx')))
+
+    def _quantize_mx_inputs(self) -> None:
+        """An MXFP4 product reads its activation in MXFP4: one quantisation per tensor, ahead of its first reader.  With
+        ``fuse_mx_chain``, a tensor that another MXFP4 product writes and only such products read is written in MXFP4 right away
+        and has no float form at all."""
+        graph = self.graph
+        kinds = ('dense_mx', 'gated_dense_mx')
+        if not any(op['kind'] in kinds for op in self.ops):
+            return
+        by_name = {op['name']: op for op in self.ops}
+        produced = {op['out']: op for op in self.ops if op['kind'] in kinds}
+        aliased = set(self.alias) | {p for p, _, _ in self.alias.values()}
+        ops: List[Dict[str, Any]] = []
+        for op in self.ops:
+            t = op.get('lhs')
+            if op['kind'] in kinds and t not in self.mx:
+                producer = produced.get(t)
+                readers = [by_name.get(c.name, {}).get('kind') for c in graph.tensors[t].consumers]
+                if (self.fuse_mx_chain and producer is not None and all(r in kinds for r in readers) and t not in graph.output_tensor_names
+                        and t not in aliased):
+                    producer['out_mx'] = True
+                    self.fused.append(f"{producer['name']}+{t}/quantize")
+                else:
+                    ops.append({'kind': 'quantize_mx', 'name': f'{t}/quantize', 'lhs': t})
+                shape = [int(d) for d in graph.tensors[t].shape]
+                rows, cols = int(np.prod(shape[:-1], dtype=np.int64)), shape[-1]
+                torch = _torch()
+                self.mx[t] = (torch.zeros((rows, mx_pitch(cols) // 2), dtype=torch.uint8, device=self.device),
+                              torch.zeros(int(self.lib.a4c_mx_scale_bytes(rows, cols)), dtype=torch.uint8, device=self.device))
+            ops.append(op)
+        self.ops = ops
+
+    def _mx_args(self, name: str) -> Tuple[int, int, int]:
+        codes, tiles = self.mx[name]
+        return codes.data_ptr(), 2 * int(codes.shape[1]), tiles.data_ptr()
+
+    def _mx_weight_args(self, key: str) -> Tuple[int, int, int]:
+        codes, tiles = self.params[key], self.params[key + '.scales']
+        return codes.data_ptr(), 2 * int(codes.shape[1]), tiles.data_ptr()
+
+    def _mx_output_args(self, op: Dict[str, Any], rows: int) -> tuple:
+        """(pointer, type code, pitch, scales) of what an MXFP4 product writes."""
+        if op.get('out_mx'):
+            codes, ld, tiles = self._mx_args(op['out'])
+            return codes, FLOAT_CODE['mxfp4'], ld, tiles
+        y = self._view(op['out'])
+        y_off, My, N, ldy = collapse_2d(y, f"{op['name']}: output")
+        if (My, N) != (rows, op['N']):
+            raise ValueError(f"{op['name']}: shape mismatch between views (output {y.shape}).")
+        return self.ptr(y, y_off), FLOAT_CODE[op['dtype']], ldy, None
 
     def _fuse_dense_chain(self) -> None:
         """Consecutive Dense layers whose intermediates feed nothing else become one `mlp` op when the library
@@ -667,6 +739,19 @@ class Plan:
             args = (self.ptr(a, a_off), FLOAT_CODE[op['dtype']], lda, w.data_ptr(), int(w.shape[1]),
                     bias.data_ptr() if bias is not None else None, self.ptr(y, y_off), ldy, M, K, N, int(op['relu']))
             return L.a4c_dense_f, args
+        if kind == 'quantize_mx':
+            x = self._view(op['lhs'])
+            x_off, rows, cols, ldx = collapse_2d(x, f'{name}: input')
+            return L.a4c_quantize_mx, (self.ptr(x, x_off), FLOAT_CODE[x.fmt], ldx, *self._mx_args(op['lhs']), rows, cols)
+        if kind in ('dense_mx', 'gated_dense_mx'):
+            M, K, N = int(self.mx[op['lhs']][0].shape[0]), op['K'], op['N']
+            bias = lambda key: self.params[op[key]].data_ptr() if op[key] else None
+            out = self._mx_output_args(op, M)
+            if kind == 'dense_mx':
+                return L.a4c_dense_mx, (*self._mx_args(op['lhs']), *self._mx_weight_args(op['weight']), bias('bias'), *out, M, K, N,
+                                        int(op['relu']))
+            return L.a4c_gated_dense_mx, (*self._mx_args(op['lhs']), *self._mx_weight_args(op['gate']), *self._mx_weight_args(op['up']),
+                                          bias('gate_bias'), bias('up_bias'), *out, M, K, N, ACTIVATION_CODE[op['activation']])
         if kind == 'matmul_f':
             a, b, c = self._view(op['lhs']), self._view(op['rhs']), self._view(op['out'])
             a_off, ba, ar, ac, lda, sa = collapse_batched(a, f'{name}: lhs')
@@ -804,6 +889,7 @@ class Plan:
         """The lowered plan as plain data: what the CPU oracle evaluates and what a dump records."""
         ops: List[Dict[str, Any]] = []
         params: Dict[str, np.ndarray] = {}
+        kept_in_mx = {op['name'] for op in getattr(self, 'ops', ()) if op.get('out_mx')}
         for node in self.graph.nodes:
             if node.is_placeholder:
                 if 'slice_view' in node.traits:
@@ -817,10 +903,21 @@ class Plan:
                 continue
             inst = self.ctx.ir.execution.get(node.name)
             op = inst.variant.plan_op(inst)
+            if node.name in kept_in_mx:
+                op['out_mx'] = True           # this plan never rounds the result to its float type
             if op['kind'] in ('dense', 'dense_f'):
                 params[op['weight']] = inst.artifacts['weights_kn']
                 if op['bias']:
                     params[op['bias']] = inst.artifacts['packed_bias']
+            elif op['kind'] == 'dense_mx':
+                params[op['weight']] = inst.artifacts['weights_kn']
+                if op['bias']:
+                    params[op['bias']] = inst.artifacts['packed_bias']
+            elif op['kind'] == 'gated_dense_mx':
+                for role in ('gate', 'up'):
+                    params[op[role]] = inst.artifacts[f'{role}_kn']
+                    if op[f'{role}_bias']:
+                        params[op[f'{role}_bias']] = inst.artifacts[f'packed_{role}_bias']
             elif op['kind'] == 'layer_norm':
                 params[op['gamma']] = inst.artifacts['packed_gamma']
                 params[op['beta']] = inst.artifacts['packed_beta']

@@ -141,7 +141,7 @@ class HostPipeline:
                                    fuse_attention=first.fuse_attention, merge_attention_heads=first.merge_attention_heads,
                                    merge_parallel_dense=first.merge_parallel_dense,
                                    fuse_dense_chain=first.fuse_dense_chain,
-                                   dense_algo=first.dense_algo,
+                                   dense_algo=first.dense_algo, fuse_mx_chain=first.fuse_mx_chain,
                                    share_params=first))
         self.device = first.device
         graph = first.graph

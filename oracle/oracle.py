@@ -226,6 +226,52 @@ def matmul_float(a, b, *, transpose_a: bool = False, transpose_b: bool = False, 
 
 
 # --------------------------------------------------------------------------------------------
+# MXFP4 products (no counterpart in the reference)
+# --------------------------------------------------------------------------------------------
+
+def mx_round(x):
+    """The values the MXFP4 form of ``x`` stands for: blocks of 32 along the last axis, scale 2^max(floor(log2 max) - 2, -127),
+    E2M1 magnitudes 0 .5 1 1.5 2 3 4 6, nearest even, saturating."""
+    x = np.asarray(x, dtype=np.float64)
+    cols = x.shape[-1]
+    v = np.zeros((x.size // cols, (cols + 31) // 32 * 32))
+    v[:, :cols] = x.reshape(-1, cols)
+    v = v.reshape(v.shape[0], -1, 32)
+    top = np.abs(v).max(axis=2, keepdims=True)
+    e = np.maximum(np.floor(np.log2(np.where(top > 0, top, 1.0))) - 2, -127)
+    a = np.abs(v) / np.exp2(e)
+    step = np.where(a < 2, 0.5, np.where(a < 4, 1.0, 2.0))
+    q = np.minimum(np.round(a / step) * step, 6.0) * np.exp2(e)
+    return (np.sign(v) * q).reshape(v.shape[0], -1)[:, :cols].reshape(x.shape)
+
+
+def mx_activate(x, act: str):
+    if act == 'relu':
+        return np.maximum(x, 0.0)
+    if act in ('silu', 'sigmoid'):
+        s = 1.0 / (1.0 + np.exp(-x))
+        return x * s if act == 'silu' else s
+    if act == 'gelu':
+        from math import erf
+
+        return 0.5 * x * (1.0 + np.vectorize(erf, otypes=[np.float64])(x / np.sqrt(2.0)))
+    if act == 'gelu_tanh':
+        return 0.5 * x * (1.0 + np.tanh(np.sqrt(2.0 / np.pi) * (x + 0.044715 * x ** 3)))
+    return x
+
+
+def mx_product(op: dict, x, params: dict):
+    """float64 result of an MXFP4 Dense or gated Dense on the (float) activation ``x``, which it quantises first."""
+    a = mx_round(x)
+    def linear(w, b):
+        y = a @ np.asarray(params[op[w]], dtype=np.float64)
+        return y + np.asarray(params[op[b]], dtype=np.float64) if op.get(b) else y
+    if op['kind'] == 'dense_mx':
+        return mx_activate(linear('weight', 'bias'), 'relu' if op['relu'] else 'none')
+    return mx_activate(linear('gate', 'gate_bias'), op['activation']) * linear('up', 'up_bias')
+
+
+# --------------------------------------------------------------------------------------------
 # Softmax
 # --------------------------------------------------------------------------------------------
 
@@ -473,6 +519,9 @@ def run_plan(plan: dict, inputs: dict) -> dict:
             lhs = np.swapaxes(env[op['lhs']], -1, -2) if op.get('transpose_lhs', False) else env[op['lhs']]
             env[op['out']] = dense_float(lhs, params[op['weight']], params[op['bias']] if op.get('bias') else None,
                                          relu=op['relu'], fmt=op['dtype'])
+        elif kind in ('dense_mx', 'gated_dense_mx'):
+            y = mx_product(op, env[op['lhs']], params)
+            env[op['out']] = y if op.get('out_mx') else round_float(y, op['dtype'])   # out_mx: only its MXFP4 form exists
         elif kind == 'matmul_f':
             env[op['out']] = matmul_float(env[op['lhs']], env[op['rhs']], transpose_a=op.get('transpose_lhs', False),
                                           transpose_b=op.get('transpose_rhs', False), fmt=op['dtype'])
