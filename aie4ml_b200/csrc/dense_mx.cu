@@ -45,7 +45,7 @@ constexpr size_t ONE_PER_SM = 116 * 1024;
 struct Tail {
     uint64_t full[MAX_STAGES];
     uint64_t empty[MAX_STAGES];
-    uint64_t moved[MAX_STAGES];      // the stage's A scales lie in the first column
+    uint64_t moved[MAX_STAGES];      // the stage's A scales lie in the first columns
     uint64_t done;
     uint32_t tmem_base;
     volatile int abort_flag;
@@ -155,7 +155,7 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const int kb0 = (int)((long long)g.num_kb * rank / g.split), kb1 = (int)((long long)g.num_kb * (rank + 1) / g.split);
 
     // A column of TMEM holds 32 rows' scales, and an MMA reads them from a multiple of 4 columns on.  A row tile that does not
-    // begin with a scale tile has its scales moved to the first column while they are in shared memory.
+    // begin with a scale tile has its scales moved to the first columns while they are in shared memory.
     const int sf_row = (int)(m0 % mx::TILE_ROWS) / 32;
     volatile int* abort_flag = &tail->abort_flag;
     const int a_bytes = g.t * (BK / 2);
@@ -252,8 +252,11 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 155)) break;
             uint32_t* f = reinterpret_cast<uint32_t*>(smem + (size_t)(stage + 1) * g.stage_bytes - SF_BYTES) + lane * 4;
-            f[0] = f[sf_row];
-            if (g.k_tiles - 2 * kb > 1) f[mx::TILE_BYTES / 4] = f[mx::TILE_BYTES / 4 + sf_row];
+            const int halves = min(2, g.k_tiles - 2 * kb);
+            for (int h = 0; h < halves; ++h, f += mx::TILE_BYTES / 4) {
+                f[0] = f[sf_row];
+                if (g.t == 64) f[1] = f[sf_row + 1];       // rows 64-127 of the scale tile: columns 2 and 3
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&tail->moved[stage]);

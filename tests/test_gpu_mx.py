@@ -171,7 +171,8 @@ def test_quantize_is_a_projection(lib):
 # ---- Dense --------------------------------------------------------------------------------------
 
 SHAPES = [(1, 1, 1), (1, 32, 16), (3, 33, 5), (1, 4096, 200), (16, 64, 128), (17, 65, 129), (31, 255, 33), (64, 256, 256), (100, 257, 96),
-          (128, 512, 384), (129, 1000, 777), (200, 130, 1024), (256, 2048, 256), (333, 1000, 65), (385, 4096, 640)]
+          (128, 512, 384), (129, 1000, 777), (200, 130, 1024), (256, 2048, 256), (333, 1000, 65), (385, 4096, 640),
+          (190, 300, 1100), (531, 224, 1129)]
 
 
 # enough tiles of 256 x 256 (and of 256 x 128 pairs of features) that a CTA pair works through several
@@ -329,6 +330,26 @@ def test_gated_far_arguments(lib):
         got = out.get()
         assert not np.isnan(got).any()
         assert (np.abs(got - s * u)[far] <= 2.0 ** -22 * np.abs(s * u)[far]).all()
+
+
+def test_shapes_at_random(lib):
+    """Sixty shapes over the whole range of rows, K and features, each exact: whatever tile, split or kernel a size selects."""
+    rng = np.random.default_rng(20)
+    t = torch()
+    for i in range(60):
+        m, k, n = (int(round(hi ** rng.random())) for hi in (3000, 2000, 2500))
+        a, w, u = random_mx(rng, m, k), random_mx(rng, n, k), random_mx(rng, n, k)
+        x = t.from_numpy(a.values).cuda()
+        g, h = ((x @ t.from_numpy(q.values).cuda().T).cpu().numpy() for q in (w, u))      # exact in any order
+        out = Out('f32', m, n)
+        if i % 2:
+            run_dense(lib, a, w, None, out, 0)
+            want = g
+        else:
+            run_gated(lib, a, w, u, None, None, out, 'none')
+            want = (g.astype(np.float32) * h.astype(np.float32)).astype(np.float64)
+        assert np.array_equal(out.get(), want), (m, k, n, i)
+    assert lib.device_status() == 0
 
 
 # ---- as they are used ---------------------------------------------------------------------------
