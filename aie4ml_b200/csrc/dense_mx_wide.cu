@@ -52,6 +52,7 @@ constexpr int PATCH_BYTES = 32 * 64;            // per epilogue warp: 32 rows of
 constexpr int STASH_BYTES = OVERLAP * 128 * 4;  // per accumulator: the shared columns of this CTA's rows, [column][row]
 
 struct Tail {
+    float bias[4][2][128];           // per epilogue group, alternating between tiles: its columns' bias (gated: gate, then the other's)
     uint64_t full[STAGES];
     uint64_t empty[STAGES];
     uint64_t tmem_full[2];
@@ -102,10 +103,7 @@ __device__ __forceinline__ uint32_t to_words(const mx::f2* p, uint32_t* w) {
         for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
         return 0;
     }
-    uint32_t top[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 32; ++i) top[i & 3] = max(top[i & 3], __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    const uint32_t s = mx::scale_code(max(max(top[0], top[1]), max(top[2], top[3])));
+    const uint32_t s = mx::scale_code(mx::abs_max32(v));
     const mx::f2 inv = mx::both(mx::inverse_scale(s == 255u ? 0u : s));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -165,19 +163,13 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 }
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
-// adds the bias of 16 neighbouring columns from `col` on; columns beyond the row's end get none
-__device__ __forceinline__ void add_bias(mx::f2* v, const float* bias, int col, int cols) {
-    if (col + 16 <= cols && ((uintptr_t)bias & 15u) == 0) {
+// adds 16 neighbouring columns' bias, which lies in shared memory
+__device__ __forceinline__ void add_bias(mx::f2* v, const float* bias) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 b = __ldg(reinterpret_cast<const float4*>(bias + col) + i);
-            v[2 * i] = mx::add2(v[2 * i], mx::pack2(b.x, b.y));
-            v[2 * i + 1] = mx::add2(v[2 * i + 1], mx::pack2(b.z, b.w));
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = mx::add2(v[i], mx::pack2(col + 2 * i < cols ? __ldg(bias + col + 2 * i) : 0.0f, col + 2 * i + 1 < cols ? __ldg(bias + col + 2 * i + 1) : 0.0f));
+    for (int i = 0; i < 4; ++i) {
+        const float4 b = reinterpret_cast<const float4*>(bias)[i];
+        v[2 * i] = mx::add2(v[2 * i], mx::pack2(b.x, b.y));
+        v[2 * i + 1] = mx::add2(v[2 * i + 1], mx::pack2(b.z, b.w));
     }
 }
 
@@ -374,6 +366,7 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 tmem_ld16_async(taddr + (uint32_t)c, r);
             }
         };
+        const bool any_bias = g.bias[0] != nullptr || g.bias[1] != nullptr;
         uint32_t scales = 0;
         bool ok = true;
         int it = 0;
@@ -382,6 +375,13 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             int mt, nt;
             tile_coords(tile, g, mt, nt);
             const long long row0 = (long long)mt * BM + (int)rank * BM_CTA + quad * 32;
+            float* bias = tail->bias[2 * acc + half][(it >> 1) & 1];
+            if (any_bias) {                                    // fetched while the tile is still being multiplied
+                const int i = quad * 32 + lane, n = nt * OUT_COLS + half * COLS + (GATED ? i & 63 : i);
+                const float* src = GATED && i >= 64 ? g.bias[1] : g.bias[0];
+                bias[i] = src != nullptr && n < g.N ? __ldg(src + n) : 0.0f;
+                asm volatile("bar.sync %0, 128;" :: "r"(1 + 2 * acc + half) : "memory");
+            }
             if (ok) ok = mbar_wait(&tail->tmem_full[acc], (it >> 1) & 1, abort_flag, g.status, 165);
             if (!ok) continue;
             tc_fence_after();
@@ -410,12 +410,12 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     mx::f2* x = v + 8 * q;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = mx::pack2(__uint_as_float(a[2 * k]), __uint_as_float(a[2 * k + 1]));
-                    if (g.bias[0]) add_bias(x, g.bias[0], col + 16 * q, g.N);
+                    if (any_bias) add_bias(x, bias + 32 * p + 16 * q);
                     if (GATED) {
                         mx::f2 y[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) y[k] = mx::pack2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
-                        if (g.bias[1]) add_bias(y, g.bias[1], col + 16 * q, g.N);
+                        if (any_bias) add_bias(y, bias + 64 + 32 * p + 16 * q);
                         mx::activate_pairs<8>(x, g.act);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) x[k] = mx::mul2(x[k], y[k]);

@@ -41,6 +41,22 @@ __device__ __forceinline__ float scale_value(uint32_t s) {
     return __uint_as_float(s == 0u ? 0x00400000u : (s == 255u ? 0x7FC00000u : s << 23));
 }
 
+// Largest magnitude of 32 values as float bits; a NaN wins (scale_code then finds it)
+__device__ __forceinline__ uint32_t abs_max32(const float* v) {
+    float m[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        m[k] = fabsf(v[8 * k]);
+#pragma unroll
+        for (int i = 1; i < 7; i += 2)
+            asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m[k]) : "f"(fabsf(v[8 * k + i])), "f"(fabsf(v[8 * k + i + 1])));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m[k]) : "f"(fabsf(v[8 * k + 7])));
+    }
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m[0]) : "f"(m[1]), "f"(m[2]));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m[0]) : "f"(m[3]));
+    return __float_as_uint(m[0]) & 0x7FFFFFFFu;
+}
+
 // Eight scaled values -> eight E2M1 codes, element 0 in the lowest nibble.  Round to nearest even, saturating at 6.
 __device__ __forceinline__ uint32_t pack_e2m1(const float* v) {
     uint32_t w;
@@ -290,19 +306,18 @@ __device__ __forceinline__ f2 inv_one_plus_exp2(f2 z) { return each2<rcp_approx>
 
 // x Phi(x) = max(x, 0) - |x| / 2 erfc(|x| / sqrt 2), erfc by formula 7.1.26 of Abramowitz and Stegun (Handbook of
 // Mathematical Functions): t (a1 + t (a2 + ...)) exp(-z^2), t = 1 / (1 + p z), absolute error at most 1.5e-7.  erff would
-// take twice the instructions, and 1 + erf cancels for negative x.
+// take twice the instructions, and 1 + erf cancels for negative x.  (The factor -1/2 is in the coefficients.)
 __device__ __forceinline__ f2 gelu2(f2 x) {
     const f2 ax = x & 0x7FFFFFFF7FFFFFFFull;
+    const f2 e = each2<exp2_approx>(mul2(mul2(x, x), both(-0.5f * LOG2E)));
     const f2 t = each2<rcp_approx>(fma2(ax, both(0.3275911f * 0.70710678118654752f), both(1.0f)));
-    f2 p = fma2(t, both(1.061405429f), both(-1.453152027f));
-    p = fma2(t, p, both(1.421413741f));
-    p = fma2(t, p, both(-0.284496736f));
-    p = fma2(t, p, both(0.254829592f));
-    const f2 e = each2<exp2_approx>(mul2(mul2(x, both(-0.5f * LOG2E)), x));
-    const f2 h = mul2(mul2(ax, both(-0.5f)), mul2(t, p));
+    f2 p = fma2(t, both(-0.5f * 1.061405429f), both(0.5f * 1.453152027f));
+    p = fma2(t, p, both(-0.5f * 1.421413741f));
+    p = fma2(t, p, both(0.5f * 0.284496736f));
+    p = fma2(t, p, both(-0.5f * 0.254829592f));
     float a, b;
     unpack2(x, a, b);
-    return fma2(h, e, pack2(a < 0.0f ? 0.0f : a, b < 0.0f ? 0.0f : b));     // a NaN stays one
+    return fma2(mul2(mul2(ax, t), p), e, pack2(fmaxf(a, 0.0f), fmaxf(b, 0.0f)));     // a NaN comes through the other terms
 }
 
 template <int ACT>
