@@ -220,7 +220,7 @@ __device__ __forceinline__ void store32(const Args& g, const CUtensorMap* map_y,
     }
 }
 
-template <bool GATED, int OUT>
+template <bool GATED, int OUT, bool BIAS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_sa,
@@ -366,7 +366,6 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 tmem_ld16_async(taddr + (uint32_t)c, r);
             }
         };
-        const bool any_bias = g.bias[0] != nullptr || g.bias[1] != nullptr;
         uint32_t scales = 0;
         bool ok = true;
         int it = 0;
@@ -376,7 +375,7 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             tile_coords(tile, g, mt, nt);
             const long long row0 = (long long)mt * BM + (int)rank * BM_CTA + quad * 32;
             float* bias = tail->bias[2 * acc + half][(it >> 1) & 1];
-            if (any_bias) {                                    // fetched while the tile is still being multiplied
+            if (BIAS) {                                    // fetched while the tile is still being multiplied
                 const int i = quad * 32 + lane, n = nt * OUT_COLS + half * COLS + (GATED ? i & 63 : i);
                 const float* src = GATED && i >= 64 ? g.bias[1] : g.bias[0];
                 bias[i] = src != nullptr && n < g.N ? __ldg(src + n) : 0.0f;
@@ -410,12 +409,12 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     mx::f2* x = v + 8 * q;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = mx::pack2(__uint_as_float(a[2 * k]), __uint_as_float(a[2 * k + 1]));
-                    if (any_bias) add_bias(x, bias + 32 * p + 16 * q);
+                    if (BIAS) add_bias(x, bias + 32 * p + 16 * q);
                     if (GATED) {
                         mx::f2 y[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) y[k] = mx::pack2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
-                        if (any_bias) add_bias(y, bias + 64 + 32 * p + 16 * q);
+                        if (BIAS) add_bias(y, bias + 64 + 32 * p + 16 * q);
                         mx::activate_pairs<8>(x, g.act);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) x[k] = mx::mul2(x[k], y[k]);
@@ -442,12 +441,16 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem_base), "r"((uint32_t)TMEM_COLS) : "memory");
 }
 
+template <bool GATED, int OUT, bool BIAS>
+cudaError_t launch_one(const CUtensorMap* m, const Args& g, int grid, cudaStream_t s) {
+    static tc::SmemOptIn opt_in;
+    const cudaError_t e = opt_in.ensure(dense_mx_wide_kernel<GATED, OUT, BIAS>, SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    return mx::launch_serialized(dense_mx_wide_kernel<GATED, OUT, BIAS>, (unsigned)grid, NUM_THREADS, SMEM_BYTES, 0, s, m[0], m[1], m[2], m[3], m[4], m[5], m[6], g);
+}
 template <bool GATED, int OUT>
 cudaError_t launch(const CUtensorMap* m, const Args& g, int grid, cudaStream_t s) {
-    static tc::SmemOptIn opt_in;
-    const cudaError_t e = opt_in.ensure(dense_mx_wide_kernel<GATED, OUT>, SMEM_BYTES);
-    if (e != cudaSuccess) return e;
-    return mx::launch_serialized(dense_mx_wide_kernel<GATED, OUT>, (unsigned)grid, NUM_THREADS, SMEM_BYTES, 0, s, m[0], m[1], m[2], m[3], m[4], m[5], m[6], g);
+    return g.bias[0] || g.bias[1] ? launch_one<GATED, OUT, true>(m, g, grid, s) : launch_one<GATED, OUT, false>(m, g, grid, s);
 }
 
 }  // namespace
