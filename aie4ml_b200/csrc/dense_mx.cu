@@ -35,6 +35,7 @@ constexpr int BK = 256;                       // K values per stage (128 bytes o
 constexpr int W_BYTES = BN * BK / 2;
 constexpr int SF_BYTES = 2 * mx::TILE_BYTES;  // scales of 128 rows x 256 values
 constexpr int NUM_THREADS = 192;
+constexpr int EPI_THREADS = 128;
 constexpr int MAX_STAGES = 12;
 constexpr int MAX_GATED_STAGES = 10;
 constexpr int MAX_SPLIT = 8;                  // portable cluster size
@@ -64,8 +65,8 @@ struct Args {
     int t;                           // rows of A per tile: 16, 32, 64 or 128
     int split, log_split;            // CTAs per tile (cluster size), a power of two
     int num_n_tiles;
-    int stages, stage_bytes;         // the partial sums of a split reduction lie behind the stages
-    int part_bytes;
+    int stages, stage_bytes;
+    int part_bytes;                  // behind the stages: the partial sums of a split reduction, or rows on their way to MXFP4
     int act;
     uint32_t idesc;
     int* status;
@@ -87,32 +88,42 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(a[i]);
 }
 
-// One value of row m and feature n (this lane's), complete over K; the 32 lanes of a warp hold 32 neighbouring
-// features, which for an MXFP4 output are one block.  Called by whole warps with the same m.
+// One value of row m and feature n (this lane's), complete over K
 template <int OUT>
 __device__ __forceinline__ void store_value(const Args& g, long long m, int n, float v) {
-    if (OUT == mx::KIND_BF16) {
-        if (n < g.N) reinterpret_cast<__nv_bfloat16*>(g.Y)[m * g.ldy + n] = __float2bfloat16_rn(v);
-    } else if (OUT == mx::KIND_F32) {
-        if (n < g.N) reinterpret_cast<float*>(g.Y)[m * g.ldy + n] = v;
-    } else {
-        const int lane = threadIdx.x & 31;
-        const int n0 = n - lane;
-        if (n >= g.N) v = 0.0f;
-        const uint32_t s = mx::scale_code(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu));
-        uint32_t w = s == 255u ? 0u : mx::one_e2m1(v * mx::inverse_scale(s)) << (4 * (lane & 7));
-        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 1);
-        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 2);
-        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
-        uint8_t* dst = reinterpret_cast<uint8_t*>(g.Y) + (m * g.ldy + n0) / 2;
-        const int bytes = (min(32, g.N - n0) + 1) >> 1;       // <= 0 for a block beyond the row's end, whose scale is 0
-        // lane 8 j holds the word of features 8 j .. 8 j + 7
-        if ((lane & 7) == 0) {
-            const int b0 = lane >> 1;
-            if (b0 + 4 <= bytes) *reinterpret_cast<uint32_t*>(dst + b0) = w;
-            else for (int b = b0; b < bytes; ++b) dst[b] = (uint8_t)(w >> (8 * (b - b0)));
+    if (n >= g.N) return;
+    if (OUT == mx::KIND_BF16) reinterpret_cast<__nv_bfloat16*>(g.Y)[m * g.ldy + n] = __float2bfloat16_rn(v);
+    else reinterpret_cast<float*>(g.Y)[m * g.ldy + n] = v;
+}
+
+// MXFP4 output: a lane holds one feature, a block is 32 of them.  The finished values go through shared memory, rows of 4 blocks
+// 36 floats apart (so that the 16-byte reads of a warp, 8 rows x 4 blocks, meet no bank twice), and a thread takes a whole block.
+constexpr int MX_BLOCK_PITCH = 36, MX_ROW_PITCH = 4 * MX_BLOCK_PITCH;
+__device__ __forceinline__ int mx_slot(int row, int nl) { return row * MX_ROW_PITCH + (nl >> 5) * MX_BLOCK_PITCH + (nl & 31); }
+
+// block t & 3 of row t / 4 for every t = thread, thread + 128, ...; buffered row i is row first + i * step of the tile
+__device__ __forceinline__ void store_mx(const Args& g, const float* buf, int count, long long m0, int first, int step, int n0, int thread) {
+#pragma unroll 1
+    for (int t = thread; t < 4 * count; t += EPI_THREADS) {
+        const int b = t & 3, n = n0 + 32 * b;
+        const float4* src = reinterpret_cast<const float4*>(buf + (t >> 2) * MX_ROW_PITCH + b * MX_BLOCK_PITCH);
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 q = src[i];
+            v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
         }
-        if (lane == 0) g.ys[mx::scale_offset(m, n0 >> 5, g.y_across)] = (uint8_t)s;
+        uint32_t w[4];
+        const uint32_t s = mx::quantize32(v, w);
+        const long long m = m0 + first + (long long)(t >> 2) * step;
+        uint8_t* dst = reinterpret_cast<uint8_t*>(g.Y) + (m * g.ldy + n) / 2;
+        const int bytes = (min(32, g.N - n) + 1) >> 1;        // <= 0 for a block beyond the row's end, whose scale is 0
+        if (bytes == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) if (i < bytes) dst[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+        }
+        g.ys[mx::scale_offset(m, n >> 5, g.y_across)] = (uint8_t)s;
     }
 }
 
@@ -280,6 +291,8 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (g.bias[0]) ba = __ldg(g.bias[0] + n);
         if (GATED && g.bias[1]) bu = __ldg(g.bias[1] + n);
     }
+    // rows on their way to MXFP4: over the stages, which are done with, where they are large enough
+    float* rowbuf = g.split > 1 || g.part_bytes == 0 ? reinterpret_cast<float*>(smem) : part;
     if (g.split == 1) {
         if (ok) {
 #pragma unroll 1
@@ -289,9 +302,16 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (GATED) tmem_ld16(taddr + (uint32_t)(MAX_T + c), u);
                 finish_values<GATED, 16>(g, a, u, ba, bu);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (c + i < rows) store_value<OUT>(g, m0 + c + i, n, a[i]);
+                for (int i = 0; i < 16; ++i) {
+                    if (c + i >= rows) break;
+                    if (OUT == mx::KIND_MX) rowbuf[mx_slot(c + i, nl)] = n < g.N ? a[i] : 0.0f;
+                    else store_value<OUT>(g, m0 + c + i, n, a[i]);
+                }
             }
+        }
+        if (OUT == mx::KIND_MX && warp >= 2) {
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (ok) store_mx(g, rowbuf, rows, m0, 0, 1, n0, threadIdx.x - 64);
         }
     } else {
         // row r is finished by rank r mod split; part[from][r / split][projection][feature] there
@@ -325,7 +345,12 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         if (GATED) u += p[q * per * NW * BN + BN];
                     }
                 finish_values<GATED, 1>(g, &a, &u, ba, bu);
-                if (ok) store_value<OUT>(g, m0 + r, n, a);
+                if (OUT == mx::KIND_MX) rowbuf[mx_slot(r >> g.log_split, nl)] = n < g.N ? a : 0.0f;
+                else if (ok) store_value<OUT>(g, m0 + r, n, a);
+            }
+            if (OUT == mx::KIND_MX) {
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (ok) store_mx(g, rowbuf, (rows - (int)rank + g.split - 1) >> g.log_split, m0, (int)rank, g.split, n0, threadIdx.x - 64);
             }
         }
     }
@@ -379,11 +404,13 @@ int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stre
     g.idesc = mx::make_idesc(BN, g.t);
     g.stage_bytes = nw * W_BYTES + g.t * (BK / 2) + (nw + 1) * SF_BYTES;
     const int need = (g.num_kb + g.split - 1) / g.split;
-    int stages = (SMEM_BUDGET - (g.split > 1 ? nw * g.t * BN * 4 : 0)) / g.stage_bytes;
-    if (stages > (gated ? MAX_GATED_STAGES : MAX_STAGES)) stages = gated ? MAX_GATED_STAGES : MAX_STAGES;
-    if (need < stages) stages = need;
-    g.stages = stages;
+    const int limit = gated ? MAX_GATED_STAGES : MAX_STAGES;
     g.part_bytes = g.split > 1 ? nw * g.t * BN * 4 : 0;
+    g.stages = (SMEM_BUDGET - g.part_bytes) / g.stage_bytes;
+    if (g.stages > limit) g.stages = limit;
+    if (need < g.stages) g.stages = need;
+    const int row_bytes = d.out_kind == mx::KIND_MX && g.split == 1 ? g.t * MX_ROW_PITCH * 4 : 0;
+    if (row_bytes > g.stages * g.stage_bytes) g.part_bytes = row_bytes;      // few stages: it fits beside them
     size_t smem = 1024 + (size_t)g.stages * g.stage_bytes + g.part_bytes + sizeof(Tail);
     // More than half of an SM's shared memory, so that one CTA lives on an SM at a time: the ranks of a cluster wait for
     // one another while they hold tensor memory, and two clusters that shared SMs could each wait for the other's.

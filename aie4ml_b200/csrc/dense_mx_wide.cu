@@ -103,16 +103,7 @@ __device__ __forceinline__ uint32_t to_words(const mx::f2* p, uint32_t* w) {
         for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
         return 0;
     }
-    const uint32_t s = mx::scale_code(mx::abs_max32(v));
-    const mx::f2 inv = mx::both(mx::inverse_scale(s == 255u ? 0u : s));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float q[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mx::unpack2(mx::mul2(p[4 * i + k], inv), q[2 * k], q[2 * k + 1]);
-        w[i] = s == 255u ? 0u : mx::pack_e2m1(q);
-    }
-    return s;
+    return mx::quantize32(v, w);
 }
 
 template <int OUT> struct Words { static constexpr int value = OUT == mx::KIND_BF16 ? 16 : OUT == mx::KIND_F32 ? 32 : 4; };

@@ -27,6 +27,23 @@ __device__ __forceinline__ long long scale_offset(long long row, long long block
     return ((row >> 7) * across + (block >> 2)) * TILE_BYTES + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
+// Two float32 values in a 64-bit register pair: one instruction for both, half the issue slots of an epilogue.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float lo, float hi) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ f2 both(float x) { return pack2(x, x); }
+__device__ __forceinline__ void unpack2(f2 p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float rcp_approx(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+template <float (*F)(float)>
+__device__ __forceinline__ f2 each2(f2 p) {
+    float a, b;
+    unpack2(p, a, b);
+    return pack2(F(a), F(b));
+}
+
 // Largest magnitude's float bits (sign cleared; NaN and infinity order above every finite value) -> scale code.
 // floor(log2) is the exponent field, 2 is the exponent of the largest E2M1 binade; subnormal and zero maxima take the
 // smallest scale.
@@ -69,14 +86,6 @@ __device__ __forceinline__ uint32_t pack_e2m1(const float* v) {
         : "=r"(w) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return w;
 }
-// one value; the codes' byte stands in all four
-__device__ __forceinline__ uint32_t one_e2m1(float v) {
-    uint32_t w;
-    asm("{\n\t.reg .b8 b0;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-        "mov.b32 %0, {b0, b0, b0, b0};\n\t}" : "=r"(w) : "f"(v), "f"(0.0f));
-    return w & 15u;
-}
 // Eight E2M1 codes -> float (exact)
 __device__ __forceinline__ void unpack_e2m1(uint32_t w, float* v) {
     uint32_t h[4];
@@ -98,6 +107,20 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t w, float* v) {
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// 32 float32 values -> their codes and scale
+__device__ __forceinline__ uint32_t quantize32(const float* v, uint32_t* w) {
+    const uint32_t s = scale_code(abs_max32(v));
+    const f2 inv = both(inverse_scale(s == 255u ? 0u : s));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float q[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) unpack2(mul2(pack2(v[8 * i + 2 * k], v[8 * i + 2 * k + 1]), inv), q[2 * k], q[2 * k + 1]);
+        w[i] = s == 255u ? 0u : pack_e2m1(q);
+    }
+    return s;
 }
 
 // ---- block-scaled tensor-core instructions ------------------------------------------------------
@@ -281,23 +304,6 @@ inline bool make_out_map(CUtensorMap* map, void* base, int kind, long long rows,
 
 // ---- activations of the gated Dense -------------------------------------------------------------
 constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_SIGMOID = 5, ACT_COUNT = 6;
-
-// Two float32 values in a 64-bit register pair: one instruction for both, half the issue slots of an epilogue.
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pack2(float lo, float hi) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
-__device__ __forceinline__ f2 both(float x) { return pack2(x, x); }
-__device__ __forceinline__ void unpack2(f2 p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
-__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-__device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-__device__ __forceinline__ float rcp_approx(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-template <float (*F)(float)>
-__device__ __forceinline__ f2 each2(f2 p) {
-    float a, b;
-    unpack2(p, a, b);
-    return pack2(F(a), F(b));
-}
 
 constexpr float LOG2E = 1.4426950408889634f;
 
