@@ -446,11 +446,16 @@ cudaError_t launch(const CUtensorMap* m, const Args& g, int grid, cudaStream_t s
 
 }  // namespace
 
-// Tiles of the pair kernel; below about a wave of pairs the smaller tiles of dense_mx.cu spread better over the SMs.
-bool a4c_dense_mx_wide_wanted(const A4cMxDense& d, int sms) {
-    const long long cols = d.wu != nullptr ? 128 : 256;
+// When the pair kernel is the faster one (148 SMs; microseconds on the device, pair kernel against dense_mx.cu):
+//   Dense, 32 tiles: 5.4 / 7.5 at K = 256, 10.4 / 13.2 at K = 4096;  16 tiles: 5.3 / 5.1 at K = 256, 6.2 / 6.6 at 1024,
+//   10.2 / 11.7 at 4096;  8 tiles: 5.3 / 3.7, 6.3 / 5.1, 10.2 / 9.9.
+//   Gated, 64 tiles: 6.2 / 6.8 at K = 256, 11.9 / 15.0 at 4096;  32 tiles: 5.5 / 4.9, 10.6 / 12.4;  8 tiles: 5.4 / 3.7, 10.4 / 10.9.
+// Up to 128 rows half of each 256-row tile would be empty.
+bool a4c_dense_mx_wide_wanted(const A4cMxDense& d) {
+    const bool gated = d.wu != nullptr;
+    const long long cols = gated ? 128 : 256;
     const long long tiles = ((d.M + BM - 1) / BM) * ((d.N + cols - 1) / cols);
-    return tiles * 2 >= sms / 2 && d.M > 128;
+    return d.M > 128 && (tiles >= (gated ? 40 : 24) || (tiles >= 16 && d.K >= 1024));
 }
 
 int a4c_launch_dense_mx_wide(const A4cMxDense& d, int sms, int* status_word, cudaStream_t stream) {
