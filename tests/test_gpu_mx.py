@@ -433,3 +433,114 @@ def test_rows_do_not_depend_on_their_batch(lib):
     run_dense(lib, a, w, None, big, 0)
     run_dense(lib, one, w, None, small, 0)
     assert np.array_equal(big.get()[:1], small.get())
+
+
+@pytest.mark.parametrize('m', [40, 300])
+@pytest.mark.parametrize('gated', [False, True])
+def test_nan_and_overflow_in_an_mxfp4_output(lib, m, gated):
+    """A block whose float results hold a NaN or an infinity is a NaN block; its neighbours are what they were.  m = 40 takes the
+    small tiles, 300 x 6000 the pair kernel."""
+    n, k = 6000, 64
+    rng = np.random.default_rng(m + gated)
+    a, w, u = random_mx(rng, m, k), random_mx(rng, n, k), random_mx(rng, n, k, 127, 127)
+    a.np_scales[5] = 255                            # row 5: NaN everywhere
+    w.np_scales[70] = 255                           # column 70: NaN
+    w.np_scales[200], w.np_codes[200] = 250, 7      # column 200: beyond float32 in rows whose sum does not cancel
+    a, w = Mx(a.np_codes, a.np_scales), Mx(w.np_codes, w.np_scales)
+    with np.errstate(over='ignore', invalid='ignore'):
+        want = (a.values @ w.values.T).astype(np.float32)
+        if gated:
+            want = want * (a.values @ u.values.T).astype(np.float32)
+    out = Out('mx', m, n)
+    if gated:
+        run_gated(lib, a, w, u, None, None, out, 'none')
+    else:
+        run_dense(lib, a, w, None, out, 0)
+    codes, scales = out.get()
+    want_codes, want_scales = R.quantize(want.astype(np.float64))
+    sure = np.ones_like(want_scales, dtype=bool)
+    sure[:, 200 // 32] = False                      # a partial sum may pass float32's range where the whole does not
+    assert np.array_equal(scales[sure], want_scales[sure])
+    assert (scales[5] == 255).all() and (scales[:, 2] == 255).all()
+    keep = np.repeat(sure & (want_scales != 255), 32, axis=1)[:, :n]
+    assert np.array_equal(R.values(codes, np.where(scales == 255, 0, scales))[keep], R.values(want_codes, np.where(want_scales == 255, 0, want_scales))[keep])
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'f32'])
+def test_wide_output_at_any_address(lib, kind):
+    """An output whose base is not 16-byte aligned, in the kernel that otherwise stores by bulk copies."""
+    t = torch()
+    rng = np.random.default_rng(4)
+    a, w = random_mx(rng, 300, 96), random_mx(rng, 6400, 96)
+    td = {'bf16': t.bfloat16, 'f32': t.float32}[kind]
+    store = t.full((300 * 6400 + 16,), -7.0, dtype=td, device='cuda')
+    y = store[1:1 + 300 * 6400]
+    lib.check(lib.load().a4c_dense_mx(*a.args, *w.args, None, y.data_ptr(), F[kind], 6400, None, 300, 96, 6400, 0, stream()), 'dense')
+    want = a.values @ w.values.T
+    assert np.array_equal(y.view(300, 6400).double().cpu().numpy(), bf16_round(want) if kind == 'bf16' else want)
+    assert float(store[0]) == -7.0 and (store[1 + 300 * 6400:] == -7.0).all()
+
+
+def test_offsets_beyond_32_bits(lib):
+    """5 GB activations: the last rows of quantisation and of both products are what they are on their own."""
+    t = torch()
+    L = lib.load()
+    rows, cols, n = 700000, 4096, 128
+    x = t.empty(rows, cols, dtype=t.bfloat16, device='cuda')
+    tail = t.randn(500, cols, device='cuda').bfloat16()
+    x.zero_()
+    x[-500:] = tail
+    q = t.empty(rows, cols // 2, dtype=t.uint8, device='cuda')
+    s = t.empty(L.a4c_mx_scale_bytes(rows, cols), dtype=t.uint8, device='cuda')
+    lib.check(L.a4c_quantize_mx(x.data_ptr(), 0, cols, q.data_ptr(), cols, s.data_ptr(), rows, cols, stream()), 'quantize')
+    codes, scales = R.quantize(tail.double().cpu().numpy())
+    got = q[-500:].cpu().numpy()
+    assert np.array_equal(np.stack([got & 15, got >> 4], 2).reshape(500, -1), codes)
+    assert np.array_equal(R.untile_scales(s.cpu().numpy(), rows, cols)[-500:], scales)
+    lib.check(L.a4c_dequantize_mx(q.data_ptr(), cols, s.data_ptr(), x.data_ptr(), 0, cols, rows, cols, stream()), 'dequantize')
+    assert np.array_equal(x[-500:].double().cpu().numpy(), R.values(codes, scales)) and not x[:-500].any()
+    # as the activation of a product, and as its output (K small, N large)
+    rng = np.random.default_rng(8)
+    w = random_mx(rng, n, cols, spare=0)
+    y = t.empty(rows, n, dtype=t.float32, device='cuda')
+    lib.check(L.a4c_dense_mx(q.data_ptr(), cols, s.data_ptr(), *w.args, None, y.data_ptr(), 1, n, None, rows, cols, n, 0, stream()), 'dense')
+    v = R.values(codes, scales)
+    err = np.abs(y[-500:].double().cpu().numpy() - v @ w.values.T)
+    assert (err <= (cols + 2) * 2.0 ** -23 * (np.abs(v) @ np.abs(w.values.T))).all() and not y[:-500].any()
+    a = random_mx(rng, 600, 32, spare=0)
+    big = random_mx(rng, cols, 32, spare=0)
+    rep = t.empty(rows, 16, dtype=t.uint8, device='cuda')
+    rep[:] = a.codes.repeat(rows // 600 + 1, 1)[:rows]
+    # 600 rows repeat, scales are the same throughout: a constant tensor of 2^0
+    ones = t.full((L.a4c_mx_scale_bytes(rows, 32),), 0, dtype=t.uint8, device='cuda')
+    ones.view(-1, 32, 4, 4)[..., 0] = 127
+    lib.check(L.a4c_dense_mx(rep.data_ptr(), 32, ones.data_ptr(), *big.args, None, x.data_ptr(), 0, cols, None, rows, 32, cols, 0, stream()), 'dense')
+    last = rows - 1 - (rows - 1) % 600
+    want = bf16_round(R.VALUES[a.np_codes[:rows - last]] @ big.values.T)
+    assert np.array_equal(x[last:].double().cpu().numpy(), want)
+    assert t.equal(x[:600], x[600 * 1000:600 * 1001])
+    assert lib.device_status() == 0
+
+
+def test_two_graphs_in_flight(lib):
+    """Two captured blocks on two streams at once: there is no memory between calls that they could share."""
+    t = torch()
+    rng = np.random.default_rng(12)
+    sets = []
+    for i, m in enumerate((9, 200)):
+        a, w, u = random_mx(rng, m, 640), random_mx(rng, 500, 640), random_mx(rng, 500, 640)
+        out = Out('f32', m, 500)
+        st, g = t.cuda.Stream(), t.cuda.CUDAGraph()
+        run_gated(lib, a, w, u, None, None, out, 'none')
+        t.cuda.synchronize()
+        with t.cuda.graph(g, stream=st):
+            for _ in range(6):
+                run_gated(lib, a, w, u, None, None, out, 'none')
+        sets.append((st, g, out, (a.values @ w.values.T).astype(np.float32) * (a.values @ u.values.T).astype(np.float32), (a, w, u)))
+    for _ in range(5):
+        for st, g, *_ in sets:
+            with t.cuda.stream(st):
+                g.replay()
+    t.cuda.synchronize()
+    for _, _, out, want, _ in sets:
+        assert np.array_equal(out.get(), want.astype(np.float64))
