@@ -303,9 +303,8 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 finish_values<GATED, 16>(g, a, u, ba, bu);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    if (c + i >= rows) break;
-                    if (OUT == mx::KIND_MX) rowbuf[mx_slot(c + i, nl)] = n < g.N ? a[i] : 0.0f;
-                    else store_value<OUT>(g, m0 + c + i, n, a[i]);
+                    if (OUT == mx::KIND_MX) rowbuf[mx_slot(c + i, nl)] = n < g.N ? a[i] : 0.0f;      // g.t rows have room
+                    else if (c + i < rows) store_value<OUT>(g, m0 + c + i, n, a[i]);
                 }
             }
         }
