@@ -291,11 +291,6 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             bool ok = true;
             for (int tile = pair; ok && tile < num_tiles; tile += num_pairs, ++it) {
                 const int acc = it & 1;
-                ok = mbar_wait_spin(&tail->tmem_empty[acc], ((it >> 1) & 1) ^ 1u, abort_flag, g.status, 162);
-                if (ok && it > 0)
-                    ok = mbar_wait_spin(&tail->overlap_free[acc ^ 1], ((it - 1) >> 1) & 1, abort_flag, g.status, 163);
-                if (!ok) break;
-                tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(acc ? ACC1 : 0);
                 for (int kb = 0; kb < g.num_kb; ++kb, ++step) {
                     ok = mbar_wait(&tail->full[stage], phase, abort_flag, g.status, 164);
@@ -316,6 +311,15 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                             mx::copy_scales_pair(sf + (uint32_t)(8 + h * 8), t + (uint64_t)(SF_BYTES >> 4));
                             mx::copy_scales_pair(sf + (uint32_t)(12 + h * 8), t + (uint64_t)(2 * SF_BYTES >> 4));
                         }
+                    }
+                    __syncwarp();
+                    if (kb == 0) {               // the tile's first scales are on their way while the epilogue frees the accumulator
+                        ok = mbar_wait_spin(&tail->tmem_empty[acc], ((it >> 1) & 1) ^ 1u, abort_flag, g.status, 162) &&
+                             (it == 0 || mbar_wait_spin(&tail->overlap_free[acc ^ 1], ((it - 1) >> 1) & 1, abort_flag, g.status, 163));
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    if (mx::elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             if (k >= steps) break;
