@@ -314,8 +314,8 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     }
                     __syncwarp();
                     if (kb == 0) {               // the tile's first scales are on their way while the epilogue frees the accumulator
-                        ok = mbar_wait_spin(&tail->tmem_empty[acc], ((it >> 1) & 1) ^ 1u, abort_flag, g.status, 162) &&
-                             (it == 0 || mbar_wait_spin(&tail->overlap_free[acc ^ 1], ((it - 1) >> 1) & 1, abort_flag, g.status, 163));
+                        ok = mbar_wait(&tail->tmem_empty[acc], ((it >> 1) & 1) ^ 1u, abort_flag, g.status, 162) &&
+                             (it == 0 || mbar_wait(&tail->overlap_free[acc ^ 1], ((it - 1) >> 1) & 1, abort_flag, g.status, 163));
                         if (!ok) break;
                         tc_fence_after();
                     }
