@@ -49,7 +49,7 @@ constexpr int EPI_WARPS = 16;
 constexpr int EPI_WARP0 = 2;                   // first epilogue warp
 constexpr int NUM_THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
 constexpr int PATCH_BYTES = 32 * 64;            // per epilogue warp: 32 rows of a TMA store's box
-constexpr int STASH_BYTES = OVERLAP * 128 * 4;  // per accumulator: the shared columns of this CTA's rows, [column][row]
+constexpr int STASH_BYTES = OVERLAP * 128 * 4;  // per accumulator: the shared columns of this CTA's rows
 
 struct Tail {
     float bias[4][2][128];           // per epilogue group, alternating between tiles: its columns' bias (gated: gate, then the other's)
@@ -78,14 +78,31 @@ struct Args {
     int* status;
 };
 
-// column tile fastest inside a panel of weights that stays in the L2 while the row tiles stream past
-__device__ __forceinline__ void tile_coords(int tile, const Args& g, int& mt, int& nt) {
-    const int per_panel = g.num_m_tiles * g.panel;
-    const int pz = tile / per_panel, rem = tile - pz * per_panel;
-    const int width = min(g.panel, g.num_n_tiles - pz * g.panel);
-    mt = rem / width;
-    nt = pz * g.panel + (rem - mt * width);
-}
+// The tiles of one pair, in order: column tile fastest inside a panel of weights that stays in the L2 while the row tiles stream
+// past.  With one panel the next tile's place follows by additions (two integer divisions a tile are a fifth of what a warp
+// of the epilogue issues for it at short reductions).
+struct Tiles {
+    int tile, mt, nt, step, step_m, step_n;
+    __device__ __forceinline__ Tiles(const Args& g, int pair, int num_pairs) : tile(pair), step(num_pairs) {
+        step_m = num_pairs / g.num_n_tiles;
+        step_n = num_pairs - step_m * g.num_n_tiles;
+        locate(g);
+    }
+    __device__ __forceinline__ void locate(const Args& g) {
+        const int per_panel = g.num_m_tiles * g.panel;
+        const int pz = tile / per_panel, rem = tile - pz * per_panel;
+        const int width = min(g.panel, g.num_n_tiles - pz * g.panel);
+        mt = rem / width;
+        nt = pz * g.panel + (rem - mt * width);
+    }
+    __device__ __forceinline__ void next(const Args& g) {
+        tile += step;
+        if (g.panel < g.num_n_tiles) { locate(g); return; }
+        mt += step_m;
+        nt += step_n;
+        if (nt >= g.num_n_tiles) { nt -= g.num_n_tiles; ++mt; }
+    }
+};
 
 // 32 finished neighbouring values of one row (as pairs) -> words of the output type (16 bf16, 32 f32, 4 MXFP4) and its scale
 template <int OUT>
@@ -259,11 +276,9 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-                int mt, nt;
-                tile_coords(tile, g, mt, nt);
-                const int m0 = mt * BM + (int)rank * BM_CTA;
-                const int n0 = nt * OUT_COLS;
+            for (Tiles t(g, pair, num_pairs); ok && t.tile < num_tiles; t.next(g)) {
+                const int m0 = t.mt * BM + (int)rank * BM_CTA;
+                const int n0 = t.nt * OUT_COLS;
                 const CUtensorMap* mw = GATED && rank ? &map_u : &map_w;
                 const int nw = GATED ? n0 : n0 + (int)rank * BN_CTA;
                 const int gw = n0 / mx::TILE_ROWS;
@@ -345,7 +360,9 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         // accumulator 1 (first half; gated: of the gate).  Their group has them in `stash`, every thread its own row's.
         const bool holder = half == 1 - acc;
         const int shared0 = acc ? 0 : BN - OVERLAP;            // first shared column of the accumulator
-        float* stash = reinterpret_cast<float*>(patches + EPI_WARPS * PATCH_BYTES + acc * STASH_BYTES) + quad * 32 + lane;
+        // (16-byte piece p of row r at p ^ (r / 2 & 3): rows are 12 pieces apart, so eight lanes then meet eight different bank groups)
+        uint8_t* stash = patches + EPI_WARPS * PATCH_BYTES + acc * STASH_BYTES + (quad * 32 + lane) * (OVERLAP * 4);
+        const uint32_t swz = (uint32_t)(lane >> 1) & 3u;
         static_assert(OVERLAP % 16 == 0 && OVERLAP <= COLS, "the shared columns are whole pieces of one group");
         auto release = [&](uint64_t* bar) {                    // this warp has read its part
             tc_fence_before();
@@ -355,8 +372,12 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         // 16 columns of the accumulator, from `c` on, of this thread's row
         auto take = [&](int c, uint32_t* r) {
             if (holder && (acc ? c < OVERLAP : c >= BN - OVERLAP)) {
+                const uint8_t* at = stash + (c - shared0) * 4;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(stash[(c - shared0 + i) * 128]);
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 q = *reinterpret_cast<const uint4*>(at + ((i ^ swz) << 4));
+                    r[4 * i] = q.x; r[4 * i + 1] = q.y; r[4 * i + 2] = q.z; r[4 * i + 3] = q.w;
+                }
             } else {
                 tmem_ld16_async(taddr + (uint32_t)c, r);
             }
@@ -364,11 +385,10 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         uint32_t scales = 0;
         bool ok = true;
         int it = 0;
-        for (int tile = pair; tile < num_tiles; tile += num_pairs, ++it) {
+        for (Tiles t(g, pair, num_pairs); t.tile < num_tiles; t.next(g), ++it) {
             if ((it & 1) != acc) continue;
-            int mt, nt;
-            tile_coords(tile, g, mt, nt);
-            const long long row0 = (long long)mt * BM + (int)rank * BM_CTA + quad * 32;
+            const int nt = t.nt;
+            const long long row0 = (long long)t.mt * BM + (int)rank * BM_CTA + quad * 32;
             float* bias = tail->bias[2 * acc + half][(it >> 1) & 1];
             if (BIAS) {                                    // fetched while the tile is still being multiplied
                 const int i = quad * 32 + lane, n = nt * OUT_COLS + half * COLS + (GATED ? i & 63 : i);
@@ -387,7 +407,8 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 for (int i = 0; i < OVERLAP / 16; ++i) tmem_ld_wait16(r + 16 * i);
                 release(&tail->overlap_free[acc]);
 #pragma unroll
-                for (int i = 0; i < OVERLAP; ++i) stash[i * 128] = __uint_as_float(r[i]);
+                for (int i = 0; i < OVERLAP / 4; ++i)
+                    *reinterpret_cast<uint4*>(stash + (i >> 2) * 64 + (((i & 3) ^ swz) << 4)) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
             }
 #pragma unroll 1
             for (int p = 0; p < COLS / 32; ++p) {              // 32 outputs at a time
