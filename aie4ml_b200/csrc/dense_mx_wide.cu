@@ -171,6 +171,10 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 }
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
+__device__ __forceinline__ void cp_async4_or_zero(void* dst, const void* src, bool any) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(smem_u32(dst)), "l"(src), "r"(any ? 4 : 0) : "memory");
+}
+
 // adds 16 neighbouring columns' bias, which lies in shared memory
 __device__ __forceinline__ void add_bias(mx::f2* v, const float* bias) {
 #pragma unroll
@@ -384,19 +388,27 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         };
         uint32_t scales = 0;
         bool ok = true;
-        int it = 0;
-        for (Tiles t(g, pair, num_pairs); t.tile < num_tiles; t.next(g), ++it) {
-            if ((it & 1) != acc) continue;
+        Tiles t(g, pair + acc * num_pairs, 2 * num_pairs);
+        // the bias of a tile's columns is on its way while the group converts the tile before (fetched at the tile's start it cost
+        // a gated 65536 x 256 x 2*1024 5.6 us)
+        auto fetch_bias = [&](int j) {
+            const int i = quad * 32 + lane, n = t.nt * OUT_COLS + half * COLS + (GATED ? i & 63 : i);
+            const float* src = GATED && i >= 64 ? g.bias[1] : g.bias[0];
+            const bool any = src != nullptr && n < g.N;
+            cp_async4_or_zero(&tail->bias[2 * acc + half][j & 1][i], any ? src + n : g.bias[0] ? g.bias[0] : g.bias[1], any);
+        };
+        if (BIAS && t.tile < num_tiles) fetch_bias(0);
+        for (int j = 0; t.tile < num_tiles; ++j) {
             const int nt = t.nt;
             const long long row0 = (long long)t.mt * BM + (int)rank * BM_CTA + quad * 32;
-            float* bias = tail->bias[2 * acc + half][(it >> 1) & 1];
-            if (BIAS) {                                    // fetched while the tile is still being multiplied
-                const int i = quad * 32 + lane, n = nt * OUT_COLS + half * COLS + (GATED ? i & 63 : i);
-                const float* src = GATED && i >= 64 ? g.bias[1] : g.bias[0];
-                bias[i] = src != nullptr && n < g.N ? __ldg(src + n) : 0.0f;
+            const float* bias = tail->bias[2 * acc + half][j & 1];
+            t.next(g);
+            if (BIAS) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("bar.sync %0, 128;" :: "r"(1 + 2 * acc + half) : "memory");
+                if (t.tile < num_tiles) fetch_bias(j + 1);
             }
-            if (ok) ok = mbar_wait(&tail->tmem_full[acc], (it >> 1) & 1, abort_flag, g.status, 165);
+            if (ok) ok = mbar_wait(&tail->tmem_full[acc], j & 1, abort_flag, g.status, 165);
             if (!ok) continue;
             tc_fence_after();
             if (holder) {
