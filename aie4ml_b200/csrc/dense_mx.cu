@@ -153,7 +153,7 @@ dense_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     constexpr int TMEM_COLS = 512;
     static_assert(SF0 + (GATED ? MAX_GATED_STAGES : MAX_STAGES) * SF_COLS <= TMEM_COLS, "a set of scale columns per stage");
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);      // by an offset: a pointer made from an integer is no longer known to be shared memory
     float* part = reinterpret_cast<float*>(smem + (size_t)g.stages * g.stage_bytes);
     Tail* tail = reinterpret_cast<Tail*>(smem + (size_t)g.stages * g.stage_bytes + g.part_bytes);
 
