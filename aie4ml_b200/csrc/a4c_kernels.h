@@ -39,7 +39,7 @@ struct A4cMxDense {
     int act;                                                 // a plain Dense knows none (0) and ReLU (1)
 };
 int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stream);
-bool a4c_dense_mx_wide_wanted(const A4cMxDense& d);      // whether the CTA-pair kernel is the faster one
+bool a4c_dense_mx_wide_wanted(const A4cMxDense& d, int sms);   // whether the CTA-pair kernel is the faster one
 int a4c_launch_dense_mx_wide(const A4cMxDense& d, int sms, int* status_word, cudaStream_t stream);
 
 // tcgen05 / TMA / TMEM int8 GEMM: A [M,K] K-contiguous, Wt [N,K] K-contiguous.

@@ -383,7 +383,7 @@ int a4c_launch_dense_mx(const A4cMxDense& d, int* status_word, cudaStream_t stre
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (a4c_dense_mx_wide_wanted(d)) return a4c_launch_dense_mx_wide(d, sms, status_word, stream);
+    if (a4c_dense_mx_wide_wanted(d, sms)) return a4c_launch_dense_mx_wide(d, sms, status_word, stream);
     Args g;
     g.sa = d.sa; g.sw[0] = d.sw; g.sw[1] = d.su; g.bias[0] = d.bias; g.bias[1] = d.bias_u;
     g.Y = d.y; g.ldy = d.ldy; g.ys = d.ys; g.y_across = mx::tiles_across(d.N);

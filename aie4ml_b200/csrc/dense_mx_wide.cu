@@ -494,16 +494,18 @@ cudaError_t launch(int out_kind, const CUtensorMap* m, const Args& g, int grid, 
 
 }  // namespace
 
-// When the pair kernel is the faster one (148 SMs; microseconds on the device, pair kernel against dense_mx.cu):
-//   Dense, 32 tiles: 5.4 / 7.5 at K = 256, 10.4 / 13.2 at K = 4096;  16 tiles: 5.3 / 5.1 at K = 256, 6.2 / 6.6 at 1024,
-//   10.2 / 11.7 at 4096;  8 tiles: 5.3 / 3.7, 6.3 / 5.1, 10.2 / 9.9.
-//   Gated, 64 tiles: 6.2 / 6.8 at K = 256, 11.9 / 15.0 at 4096;  32 tiles: 5.5 / 4.9, 10.6 / 12.4;  8 tiles: 5.4 / 3.7, 10.4 / 10.9.
+// When the pair kernel is the faster one (microseconds on the device, pair kernel / dense_mx.cu; `ctas` are the latter's tiles of
+// 128 rows and features):
+//   Dense: once those are more than one per SM.  144 of them: 5.5 / 4.0 at K = 256, 6.6 / 5.4 at 1024, 29.9 / 25.7 at 16384;
+//   160: 5.8 / 7.3, 6.9 / 9.9, 30.1 / 48.6.
+//   Gated: once they are too many to be cut into smaller row tiles (half the SMs).  64: 5.3 / 4.5 at K = 256, 5.6 / 5.2 at 512;
+//   80: 5.5 / 5.8, 6.0 / 6.6.  With a reduction long enough to use the pair's faster main loop earlier than that: 64: 6.4 / 6.6 at
+//   K = 1024, 16.1 / 19.3 at 8192;  48: 6.3 / 6.5, 16.1 / 19.0;  32: 6.3 / 5.5, 16.0 / 17.4.
 // Up to 128 rows half of each 256-row tile would be empty.
-bool a4c_dense_mx_wide_wanted(const A4cMxDense& d) {
-    const bool gated = d.wu != nullptr;
-    const long long cols = gated ? 128 : 256;
-    const long long tiles = ((d.M + BM - 1) / BM) * ((d.N + cols - 1) / cols);
-    return d.M > 128 && (tiles >= (gated ? 40 : 24) || (tiles >= 16 && d.K >= 1024));
+bool a4c_dense_mx_wide_wanted(const A4cMxDense& d, int sms) {
+    const long long ctas = ((d.M + 127) / 128) * ((d.N + 127) / 128);
+    if (d.M <= 128) return false;
+    return d.wu == nullptr ? ctas > sms : ctas * 2 > sms || (ctas * 4 > sms && d.K >= 1024);
 }
 
 int a4c_launch_dense_mx_wide(const A4cMxDense& d, int sms, int* status_word, cudaStream_t stream) {

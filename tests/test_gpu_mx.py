@@ -316,6 +316,72 @@ def test_gated_activations(lib, act, kind):
     assert (np.abs(out.get() - want) <= tol).all()
 
 
+@pytest.mark.parametrize('act', ['silu', 'gelu', 'gelu_tanh', 'sigmoid'])
+@pytest.mark.parametrize('kind', ['bf16', 'f32', 'mx'])
+def test_gated_activations_many_rows(lib, act, kind):
+    """The same in the pair kernel, four and more tiles to a pair, each with its columns' own biases; the first rows alone then take the
+    other kernel and give the same bits (exact sums, the same arithmetic behind them)."""
+    rng = np.random.default_rng(100 + ACTS.index(act))
+    m, k, n = 4100, 64, 2500
+    a, wg, wu = random_mx(rng, m, k, 124, 125), random_mx(rng, n, k, 125, 126), random_mx(rng, n, k, 124, 126)
+    bg, bu = exact_bias(rng, n) / 8, exact_bias(rng, n) / 8
+    g, u = gated_sums(a, wg, wu, bg, bu)
+    want = R.activate(g, act) * u
+    out = Out(kind, m, n)
+    run_gated(lib, a, wg, wu, dev32(bg), dev32(bu), out, act)
+    got = out.get()
+    assert lib.device_status() == 0
+    few = Mx(a.np_codes[:37], a.np_scales[:37])
+    some = Out(kind, 37, n)
+    run_gated(lib, few, wg, wu, dev32(bg), dev32(bu), some, act)
+    first = some.get()
+    if kind == 'mx':
+        ref_codes, ref_scales = (np.concatenate(p) for p in zip(*(R.quantize(want[i:i + 512]) for i in range(0, m, 512))))
+        ref, val = R.values(ref_codes, ref_scales), R.values(*got)
+        # a result next to a border between two codes, or a block's largest next to a power of two, may go either way
+        step = 4 * np.repeat(np.exp2(ref_scales.astype(np.float64) - 127), 32, axis=1)[:, :n]
+        assert (np.abs(val - ref) <= step).all() and (val != ref).mean() < 1e-3
+        assert np.array_equal(R.values(*first), val[:37])
+        return
+    z = np.abs(g) if act != 'gelu_tanh' else np.abs(1.6 * (g + 0.044715 * g ** 3))
+    rel = (2 + 1.2 * z + 2 + 5 + 3 * z) * 2.0 ** -23
+    tol = np.minimum(rel, 1.0) * np.abs(want) + 2.0 ** -22 * (1 + np.abs(g)) * np.abs(u)
+    if kind == 'bf16':
+        tol = tol + (np.abs(want) + tol) * 2.0 ** -8
+    assert (np.abs(got - want) <= tol).all()
+    assert np.array_equal(first, got[:37])
+
+
+@pytest.mark.parametrize('which', ['gate', 'other'])
+def test_gated_one_bias_many_rows(lib, which):
+    """Only one of the two biases, several tiles to a pair, a last tile of columns beyond the features."""
+    rng = np.random.default_rng(31)
+    m, k, n = 2600, 64, 4999
+    a, wg, wu = random_mx(rng, m, k), random_mx(rng, n, k), random_mx(rng, n, k)
+    b = exact_bias(rng, n)
+    bg, bu = (b, None) if which == 'gate' else (None, b)
+    g, u = gated_sums(a, wg, wu, bg, bu)
+    out = Out('f32', m, n)
+    run_gated(lib, a, wg, wu, dev32(bg), dev32(bu), out, 'none')
+    assert np.array_equal(out.get(), (g.astype(np.float32) * u.astype(np.float32)).astype(np.float64))
+
+
+@pytest.mark.parametrize('m', [7, 700])
+@pytest.mark.parametrize('act', ['silu', 'gelu', 'gelu_tanh', 'sigmoid'])
+def test_gated_keeps_nan(lib, m, act):
+    """A NaN in either factor is a NaN in the output, and only there."""
+    rng = np.random.default_rng(m)
+    n, k = 2300, 64
+    a, wg, wu = random_mx(rng, m, k), random_mx(rng, n, k), random_mx(rng, n, k)
+    a.np_scales[4, 1], wg.np_scales[33, 0], wu.np_scales[90, 1] = 255, 255, 255
+    a, wg, wu = (Mx(q.np_codes, q.np_scales) for q in (a, wg, wu))
+    out = Out('f32', m, n)
+    run_gated(lib, a, wg, wu, None, None, out, act)
+    want = np.zeros((m, n), dtype=bool)
+    want[4, :], want[:, 33], want[:, 90] = True, True, True
+    assert np.array_equal(np.isnan(out.get()), want)
+
+
 def test_gated_far_arguments(lib):
     """Sums of +-2^14 and more: sigmoid ends at 0 and 1 without NaN."""
     rng = np.random.default_rng(77)
@@ -435,11 +501,11 @@ def test_rows_do_not_depend_on_their_batch(lib):
     assert np.array_equal(big.get()[:1], small.get())
 
 
-@pytest.mark.parametrize('m', [40, 300])
+@pytest.mark.parametrize('m', [40, 300, 600])
 @pytest.mark.parametrize('gated', [False, True])
 def test_nan_and_overflow_in_an_mxfp4_output(lib, m, gated):
     """A block whose float results hold a NaN or an infinity is a NaN block; its neighbours are what they were.  m = 40 takes the
-    small tiles, 300 x 6000 the pair kernel."""
+    small tiles, 600 x 6000 the pair kernel."""
     n, k = 6000, 64
     rng = np.random.default_rng(m + gated)
     a, w, u = random_mx(rng, m, k), random_mx(rng, n, k), random_mx(rng, n, k, 127, 127)
