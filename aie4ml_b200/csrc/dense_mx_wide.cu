@@ -24,7 +24,7 @@
 // registers every 16 bytes of a row were an L2 request of their own).  Every wait is bounded.
 //
 // Bound by the tensor pipe under the power cap: Dense 16384 x 8192 x 8192 440 us, gated 16384 x 4096 x 2*8192 450 us (5.0 and
-// 4.9 PFLOP/s); at short reductions by the epilogue's issue slots: gated 65536 x 256 x 2*1024 30 us without activation, 47 us with GELU,
+// 4.9 PFLOP/s); at short reductions by the epilogue's issue slots: gated 65536 x 256 x 2*1024 29 us without activation, 47 us with GELU,
 // 54 us to MXFP4, 70 us with both biases (a lane's row needs every column's bias: 16 bytes a lane and four columns, which
 // shared memory returns at 128 bytes a cycle).
 #include <cuda.h>
@@ -46,10 +46,10 @@ constexpr int STAGE_BYTES = 2 * CODE_BYTES + 3 * SF_BYTES;
 constexpr int STAGES = 4;
 constexpr int SF_COLS = 24;                   // A 8, weights 16
 constexpr int SF_SETS = 2;
-// What an instantiation is for: Dense, the gated Dense of one activation (ACT_*), or of any (told by the arguments).  A switch
+// What an instantiation is for: Dense, the gated Dense of one activation (ACT_*), or of the others (told by the arguments).  A switch
 // for every 16 columns keeps their arithmetic from overlapping the next columns' loads: gated 65536 x 256 x 2*1024 took
 // 51.0 us with it and 47.3 without (GELU to bf16), 55.4 and 50.7 (SiLU to MXFP4).
-constexpr int DENSE = -1, GATED_ANY = -2;
+constexpr int DENSE = -1, GATED_OTHER = -2;
 constexpr int TMEM_COLS = 512;
 constexpr int SF0 = TMEM_COLS - SF_SETS * SF_COLS;
 constexpr int ACC1 = SF0 - BN;                // second accumulator: columns ACC1 .. SF0
@@ -182,6 +182,12 @@ __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.b
 
 __device__ __forceinline__ void cp_async4_or_zero(void* dst, const void* src, bool any) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(smem_u32(dst)), "l"(src), "r"(any ? 4 : 0) : "memory");
+}
+
+template <int ACT>
+__device__ __forceinline__ void activate8(mx::f2* v) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = mx::activate2<ACT>(v[k]);
 }
 
 // adds 16 neighbouring columns' bias, which lies in shared memory
@@ -453,12 +459,13 @@ dense_mx_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 #pragma unroll
                         for (int k = 0; k < 8; ++k) y[k] = mx::pack2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
                         if (BIAS) add_bias(y, bias + 64 + 32 * p + 16 * q);
-                        if (MODE == GATED_ANY) mx::activate_pairs<8>(x, g.act);
-                        else _Pragma("unroll") for (int k = 0; k < 8; ++k) x[k] = mx::activate2<MODE>(x[k]);
+                        if (MODE != GATED_OTHER) activate8<MODE>(x);
+                        else if (g.act == mx::ACT_RELU) activate8<mx::ACT_RELU>(x);
+                        else if (g.act == mx::ACT_SIGMOID) activate8<mx::ACT_SIGMOID>(x);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) x[k] = mx::mul2(x[k], y[k]);
                     } else if (g.act == mx::ACT_RELU) {
-                        mx::activate_pairs<8>(x, mx::ACT_RELU);
+                        activate8<mx::ACT_RELU>(x);
                     }
                 }
                 if (row0 < g.M) store32<OUT>(g, &map_y, patch, row0, lane, col, p & 1, scales, v);
@@ -543,6 +550,6 @@ int a4c_launch_dense_mx_wide(const A4cMxDense& d, int sms, int* status_word, cud
                             : d.act == mx::ACT_SILU ? launch<mx::ACT_SILU>(d.out_kind, m, g, grid, stream)
                             : d.act == mx::ACT_GELU ? launch<mx::ACT_GELU>(d.out_kind, m, g, grid, stream)
                             : d.act == mx::ACT_GELU_TANH ? launch<mx::ACT_GELU_TANH>(d.out_kind, m, g, grid, stream)
-                                                         : launch<GATED_ANY>(d.out_kind, m, g, grid, stream);
+                                                         : launch<GATED_OTHER>(d.out_kind, m, g, grid, stream);
     return err == cudaSuccess ? A4C_OK : A4C_ERR_CUDA;
 }
