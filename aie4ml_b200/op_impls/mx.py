@@ -10,6 +10,7 @@ accumulation, and writes bfloat16 or float32.  ``gated_dense`` is the first half
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Any, Dict
 
@@ -82,6 +83,17 @@ def _check_bias(node: OpNode, role: str, n_out: int) -> None:
         raise ValueError(f'{node.name}: {role} requires exactly {n_out} elements, got {int(np.asarray(bias.data).size)}.')
 
 
+def _check_extents(node: OpNode, weight, lhs_shape) -> None:
+    """What the kernels are told (n_in, n_out, the output's rows and columns) is what the tensors hold."""
+    given = tuple(node.metadata.get(key) for key in ('n_in', 'n_out'))
+    if given != tuple(weight.shape):
+        raise ValueError(f'{node.name}: n_in and n_out {given} do not match the weight {tuple(weight.shape)}.')
+    out = tuple(int(d) for d in node.outputs[0].shape)
+    rows = math.prod(lhs_shape[:-1])
+    if not out or out[-1] != weight.shape[1] or math.prod(out[:-1]) != rows:
+        raise ValueError(f'{node.name}: output {out} does not hold {rows} x {weight.shape[1]} results of the input {lhs_shape}.')
+
+
 def _check_activation(node: OpNode, known) -> None:
     if node.metadata.get('activation') not in known:
         raise ValueError(f"{node.name}: unknown activation {node.metadata.get('activation')!r}; one of {sorted(known)}.")
@@ -98,6 +110,7 @@ class MxDenseFamilyResolver(FamilyResolver):
             raise ValueError(f'{node.name}: mx_dense requires a rank>=2 input, got {lhs_shape}.')
         if not weight.is_parameter or len(weight.shape) != 2 or weight.shape[0] != lhs_shape[-1]:
             raise ValueError(f'{node.name}: mx_dense needs a constant [K, N] weight that fits the input {lhs_shape}, got {weight.shape}.')
+        _check_extents(node, weight, lhs_shape)
         _check_bias(node, 'bias', int(weight.shape[1]))
         _check_activation(node, ('none', 'relu'))
 
@@ -143,6 +156,7 @@ class GatedDenseFamilyResolver(FamilyResolver):
             raise NotImplementedError(f'{node.name}: gated_dense needs constant weights.')
         if len(gate.shape) != 2 or gate.shape != up.shape or gate.shape[0] != lhs_shape[-1]:
             raise ValueError(f'{node.name}: gated_dense weights {gate.shape} and {up.shape} do not fit the input {lhs_shape}.')
+        _check_extents(node, gate, lhs_shape)
         for role in ('gate_bias', 'up_bias'):
             _check_bias(node, role, int(gate.shape[1]))
         _check_activation(node, ACTIVATION_CODE)

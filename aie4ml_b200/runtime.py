@@ -412,13 +412,21 @@ class Plan:
         codes, tiles = self.mx[name]
         return codes.data_ptr(), 2 * int(codes.shape[1]), tiles.data_ptr()
 
-    def _mx_weight_args(self, key: str) -> Tuple[int, int, int]:
-        codes, tiles = self.params[key], self.params[key + '.scales']
+    def _mx_shape(self, name: str) -> Tuple[int, int]:
+        """Rows and columns of an activation whose MXFP4 form the plan holds."""
+        return int(self.mx[name][0].shape[0]), int(self.graph.tensors[name].shape[-1])
+
+    def _mx_weight_args(self, op: Dict[str, Any], role: str) -> Tuple[int, int, int]:
+        codes, tiles = self.params[op[role]], self.params[op[role] + '.scales']
+        if tuple(codes.shape) != (op['N'], mx_pitch(op['K']) // 2):
+            raise ValueError(f"{op['name']}: packed weights {tuple(codes.shape)} are not {op['N']} rows of {op['K']} values.")
         return codes.data_ptr(), 2 * int(codes.shape[1]), tiles.data_ptr()
 
     def _mx_output_args(self, op: Dict[str, Any], rows: int) -> tuple:
         """(pointer, type code, pitch, scales) of what an MXFP4 product writes."""
         if op.get('out_mx'):
+            if self._mx_shape(op['out']) != (rows, op['N']):
+                raise ValueError(f"{op['name']}: results of {(rows, op['N'])} do not fit the output {self._mx_shape(op['out'])}.")
             codes, ld, tiles = self._mx_args(op['out'])
             return codes, FLOAT_CODE['mxfp4'], ld, tiles
         y = self._view(op['out'])
@@ -742,15 +750,19 @@ class Plan:
         if kind == 'quantize_mx':
             x = self._view(op['lhs'])
             x_off, rows, cols, ldx = collapse_2d(x, f'{name}: input')
+            if (rows, cols) != self._mx_shape(op['lhs']):
+                raise ValueError(f'{name}: shape mismatch between views (input {x.shape}, codes for {self._mx_shape(op["lhs"])}).')
             return L.a4c_quantize_mx, (self.ptr(x, x_off), FLOAT_CODE[x.fmt], ldx, *self._mx_args(op['lhs']), rows, cols)
         if kind in ('dense_mx', 'gated_dense_mx'):
-            M, K, N = int(self.mx[op['lhs']][0].shape[0]), op['K'], op['N']
+            (M, cols), K, N = self._mx_shape(op['lhs']), op['K'], op['N']
+            if cols != K:
+                raise ValueError(f'{name}: input of {cols} features for weights of {K}.')
             bias = lambda key: self.params[op[key]].data_ptr() if op[key] else None
             out = self._mx_output_args(op, M)
             if kind == 'dense_mx':
-                return L.a4c_dense_mx, (*self._mx_args(op['lhs']), *self._mx_weight_args(op['weight']), bias('bias'), *out, M, K, N,
+                return L.a4c_dense_mx, (*self._mx_args(op['lhs']), *self._mx_weight_args(op, 'weight'), bias('bias'), *out, M, K, N,
                                         int(op['relu']))
-            return L.a4c_gated_dense_mx, (*self._mx_args(op['lhs']), *self._mx_weight_args(op['gate']), *self._mx_weight_args(op['up']),
+            return L.a4c_gated_dense_mx, (*self._mx_args(op['lhs']), *self._mx_weight_args(op, 'gate'), *self._mx_weight_args(op, 'up'),
                                           bias('gate_bias'), bias('up_bias'), *out, M, K, N, ACTIVATION_CODE[op['activation']])
         if kind == 'matmul_f':
             a, b, c = self._view(op['lhs']), self._view(op['rhs']), self._view(op['out'])
