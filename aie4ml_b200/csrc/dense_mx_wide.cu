@@ -24,8 +24,8 @@
 // registers every 16 bytes of a row were an L2 request of their own).  Every wait is bounded.
 //
 // Bound by the tensor pipe under the power cap: Dense 16384 x 8192 x 8192 440 us, gated 16384 x 4096 x 2*8192 450 us (5.0 and
-// 4.9 PFLOP/s); at short reductions by the epilogue's issue slots: gated 65536 x 256 x 2*1024 29 us without activation, 47 us with GELU,
-// 54 us to MXFP4, 70 us with both biases (a lane's row needs every column's bias: 16 bytes a lane and four columns, which
+// 4.9 PFLOP/s); at short reductions by the epilogue's issue slots: gated 65536 x 256 x 2*1024 29 us without activation, 48 us with GELU,
+// 56 us to MXFP4, 70 us with both biases (a lane's row needs every column's bias: 16 bytes a lane and four columns, which
 // shared memory returns at 128 bytes a cycle).
 #include <cuda.h>
 

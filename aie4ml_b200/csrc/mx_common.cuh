@@ -310,11 +310,16 @@ constexpr float LOG2E = 1.4426950408889634f;
 // 1 / (1 + 2^z): 2^z overflows to infinity where the quotient is 0, as it should be
 __device__ __forceinline__ f2 inv_one_plus_exp2(f2 z) { return each2<rcp_approx>(add2(each2<exp2_approx>(z), both(1.0f))); }
 
-// x Phi(x) = max(x, 0) - a Phi(-a), a = |x|, and Phi(-a) = 2^Q(a): log2 Phi(-a) is so near a parabola that seven terms do (a least
-// maximum fit over 0 <= a <= 13, weighted by max(a, 1/2) Phi(-a)), with one exponential and no quotient.  Error of the result at
-// most 1.5e-7 beside the roundings; Q falls on to below -10^6 at a = 64, where the power is 0.  NaN stays NaN.  (By the rational
-// form of erfc, an exponential and a reciprocal, a gated 65536 x 256 x 2*1024 took 59 us and with this 55; erff takes twice the
-// instructions, and 1 + erf cancels for negative x.)
+// x Phi(x) = max(x, 0) - a Phi(-a), a = |x|, and Phi(-a) = 2^Q(a): log2 Phi(-a) is so near a parabola that nine terms do, with
+// one exponential and no quotient.  The coefficients are a least maximum fit (linear programming) of the result's absolute
+// error, weighted by max(a, 1/2) Phi(-a) over 0 <= a <= 13, with a relative error of at most 2^-9 (half a bf16 step) down to
+// x = -6; that is 3.0e-8 beside the roundings.  Beyond -6, where the result is smaller than 6e-9, its relative error grows to 1.
+// Q falls on to below -10^8 at a = 64, where the power is 0.  NaN stays NaN.  Against a term less, fitted without the second
+// condition (1.6e-7; 0.4 % at -5 and 1.9 % at -6): a gated 65536 x 256 x 2*1024 takes 48.4 us for 47.3, and a quarter as many
+// values of a feed-forward block's hidden tensor change their code (14 for 52 in 2*10^8; the elementary form in 32 bits: 8).  Two
+// terms more, 1.6e-8 and 2^-9 down to -10, took 52.7 us.
+// (By the rational form of erfc, an exponential and a reciprocal, it took 59 us; erff takes twice the instructions, and 1 + erf
+// cancels for negative x.)
 __device__ __forceinline__ f2 gelu2(f2 x) {
     float a, b, na, nb, pa, pb;
     unpack2(x, a, b);
@@ -323,13 +328,14 @@ __device__ __forceinline__ f2 gelu2(f2 x) {
     asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(pa) : "f"(a));
     asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(pb) : "f"(b));
     const f2 n = pack2(na, nb);
-    f2 q = fma2(n, both(6.769469678147289e-07f), both(3.816149910562672e-05f));
-    q = fma2(n, q, both(0.000773044244851917f));
-    q = fma2(n, q, both(0.00803299155086279f));
-    q = fma2(n, q, both(0.05327378213405609f));
-    q = fma2(n, q, both(-0.45891252160072327f));
-    q = fma2(n, q, both(1.1511459350585938f));
-    q = fma2(n, q, both(-0.9999991059303284f));
+    f2 q = fma2(n, both(-1.1569092066565645e-06f), both(-1.913546111609321e-05f));
+    q = fma2(n, q, both(-8.965825691120699e-05f));
+    q = fma2(n, q, both(0.0003700188244692981f));
+    q = fma2(n, q, both(0.007366466801613569f));
+    q = fma2(n, q, both(0.0527038499712944f));
+    q = fma2(n, q, both(-0.4591405689716339f));
+    q = fma2(n, q, both(1.1511132717132568f));
+    q = fma2(n, q, both(-0.9999998211860657f));
     return fma2(n, each2<exp2_approx>(q), pack2(pa, pb));
 }
 
