@@ -92,12 +92,13 @@ struct Args {
 // of the epilogue issues for it at short reductions).
 struct Tiles {
     int tile, mt, nt, step, step_m, step_n;
-    __device__ __forceinline__ Tiles(const Args& g, int pair, int num_pairs) : tile(pair), step(num_pairs) {
+    __device__ __forceinline__ Tiles(const Args& g, int pair, int num_pairs) : tile(pair), mt(0), nt(0), step(num_pairs) {
         step_m = num_pairs / g.num_n_tiles;
         step_n = num_pairs - step_m * g.num_n_tiles;
         locate(g);
     }
     __device__ __forceinline__ void locate(const Args& g) {
+        if (tile >= g.num_m_tiles * g.num_n_tiles) return;      // beyond the last one there is no panel to divide by
         const int per_panel = g.num_m_tiles * g.panel;
         const int pz = tile / per_panel, rem = tile - pz * per_panel;
         const int width = min(g.panel, g.num_n_tiles - pz * g.panel);
