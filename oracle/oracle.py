@@ -231,18 +231,20 @@ def matmul_float(a, b, *, transpose_a: bool = False, transpose_b: bool = False, 
 
 def mx_round(x):
     """The values the MXFP4 form of ``x`` stands for: blocks of 32 along the last axis, scale 2^max(floor(log2 max) - 2, -127),
-    E2M1 magnitudes 0 .5 1 1.5 2 3 4 6, nearest even, saturating."""
+    E2M1 magnitudes 0 .5 1 1.5 2 3 4 6, nearest even, saturating; a block that holds a NaN or an infinity is NaN."""
     x = np.asarray(x, dtype=np.float64)
     cols = x.shape[-1]
     v = np.zeros((x.size // cols, (cols + 31) // 32 * 32))
     v[:, :cols] = x.reshape(-1, cols)
     v = v.reshape(v.shape[0], -1, 32)
+    bad = ~np.isfinite(v).all(axis=2, keepdims=True)
+    v = np.where(bad, 0.0, v)
     top = np.abs(v).max(axis=2, keepdims=True)
-    e = np.maximum(np.floor(np.log2(np.where(top > 0, top, 1.0))) - 2, -127)
-    a = np.abs(v) / np.exp2(e)
+    e = np.maximum(np.frexp(np.where(top > 0, top, 1.0))[1] - 3, -127)      # frexp: top = m 2^e with 0.5 <= m < 1
+    a = np.ldexp(np.abs(v), -e)
     step = np.where(a < 2, 0.5, np.where(a < 4, 1.0, 2.0))
-    q = np.minimum(np.round(a / step) * step, 6.0) * np.exp2(e)
-    return (np.sign(v) * q).reshape(v.shape[0], -1)[:, :cols].reshape(x.shape)
+    q = np.ldexp(np.minimum(np.round(a / step) * step, 6.0), e)
+    return np.where(bad, np.nan, np.copysign(q, v)).reshape(v.shape[0], -1)[:, :cols].reshape(x.shape)
 
 
 def mx_activate(x, act: str):
