@@ -182,7 +182,8 @@ def mx_pitch(cols: int) -> int:
 
 def to_mx(values):
     """float ``[rows, cols]`` -> (codes uint8 ``[rows, pitch / 2]``, scale tiles uint8), as ``a4c_quantize_mx`` lays them out
-    (include/aie4ml_b200.h): scale 2^max(floor(log2 max|x|) - 2, -127), codes to nearest even, saturating at 6."""
+    (include/aie4ml_b200.h): scale 2^max(floor(log2 max|x|) - 2, -127), codes to nearest even, saturating at 6.  What is not finite
+    as a float32 makes its block NaN."""
     x = np.asarray(values, dtype=np.float64)
     if x.ndim != 2 or x.shape[0] < 1 or x.shape[1] < 1:
         raise ValueError(f'to_mx: expected a matrix, got shape {x.shape}.')
@@ -192,7 +193,8 @@ def to_mx(values):
     v = np.zeros((rows, pitch))
     v[:, :cols] = x
     v = v.reshape(rows, blocks, 32)
-    bad = ~np.isfinite(v).all(axis=2)
+    with np.errstate(over='ignore'):
+        bad = ~np.isfinite(v.astype(np.float32)).all(axis=2)
     v = np.where(bad[:, :, None], 0.0, v)
     top = np.abs(v).max(axis=2)
     exponent = np.where(top > 0, np.frexp(top)[1] - 3, -127)          # frexp: top = m 2^e with 0.5 <= m < 1
