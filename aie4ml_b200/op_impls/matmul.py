@@ -131,12 +131,24 @@ def _validate_rank_contract(node: OpNode, *, allow_batched_rhs: bool) -> None:
                              f'{rhs_batch} against lhs shape {lhs_shape}.')
 
 
+def _validate_extents(node: OpNode) -> None:
+    """The kernels read n_out rows of packed weights and n_out bias values: there have to be as many."""
+    n = int(view_shape(node, input_tensor_for_role(node, 'rhs'), 'inputs')[-1])
+    n_out = int(node.metadata.get('n_out', n))
+    if n_out > n:
+        raise ValueError(f'{node.name}: n_out {n_out} exceeds the {n} columns of the weight.')
+    bias = optional_tensor_for_role(node, 'bias')
+    if bias is not None and bias.is_parameter and int(np.asarray(bias.data).size) < n_out:
+        raise ValueError(f'{node.name}: bias has {int(np.asarray(bias.data).size)} elements for {n_out} outputs.')
+
+
 @family_resolver('dense')
 class DenseFamilyResolver(FamilyResolver):
     op_type = 'dense'
 
     def validate_structure(self, node, _device) -> None:
         _validate_rank_contract(node, allow_batched_rhs=False)
+        _validate_extents(node)
 
 
 @family_resolver('matmul')
