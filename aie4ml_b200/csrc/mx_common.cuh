@@ -236,10 +236,7 @@ __device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t adesc, uint6
         "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
         :: "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void commit_pair(uint32_t bar_cluster_addr) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar_cluster_addr) : "memory");
-}
-// the same on the barrier at this offset in both CTAs
+// arrives, when the MMAs issued so far are done, on the barrier at this offset in both CTAs
 __device__ __forceinline__ void commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  :: "r"(bar), "h"((uint16_t)3) : "memory");
@@ -303,7 +300,7 @@ inline bool make_out_map(CUtensorMap* map, void* base, int kind, long long rows,
 }
 
 // ---- activations of the gated Dense -------------------------------------------------------------
-constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_SIGMOID = 5, ACT_COUNT = 6;
+constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_SIGMOID = 5;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -367,12 +364,4 @@ __device__ __forceinline__ void activate_pairs(f2* v, int act) {
         default: break;
     }
 }
-__device__ __forceinline__ float activate(float x, int act) {
-    f2 v = both(x);
-    activate_pairs<1>(&v, act);
-    float a, b;
-    unpack2(v, a, b);
-    return a;
-}
-
 }  // namespace mx
