@@ -231,7 +231,10 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(DequantArgs g) {
 bool grid_of(long long rows, long long cols, int& quarters, unsigned& grid, unsigned& grid_cols) {
     const long long gx = (cols - 1) / COLS + 1, gy = (rows - 1) / TILE_ROWS + 1;
     if (gx > 2147483647LL / gy) return false;
-    quarters = gx * gy < 8 * 148 ? 1 : 4;
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    quarters = gx * gy < 8LL * sms ? 1 : 4;
     grid = (unsigned)(gx * gy * (quarters == 1 ? 4 : 1));
     grid_cols = (unsigned)gx;
     return true;
