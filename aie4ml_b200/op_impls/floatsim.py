@@ -22,7 +22,7 @@ from ..quant_utils import from_storage_float, pack_constant_float
 from .base import CUDA_GENERATIONS, OpImplVariant, register_variant
 from .matmul import _transposed
 from .precision import resolve_exact_storage_dtype
-from .views import view_shape
+from .views import view_data, view_shape
 
 
 def is_float_node(node: OpNode) -> bool:
@@ -82,7 +82,7 @@ class CudaFloatDenseVariant(OpImplVariant):
     def pack(self, inst: ExecutionEntry) -> Dict[str, Any]:
         node, cfg = inst.node, inst.config
         fmt = cfg.precision['output'].format
-        W = np.asarray(input_tensor_for_role(node, 'rhs').data, dtype=np.float64)
+        W = view_data(node, input_tensor_for_role(node, 'rhs'))
         W = W.reshape(-1, W.shape[-2], W.shape[-1])[-1]
         K, N = int(W.shape[0]), int(W.shape[1])
         kp = (K + 15) // 16 * 16

@@ -30,7 +30,7 @@ from .precision import (
     resolve_exact_storage_dtype,
     to_quant_intent,
 )
-from .views import is_identity, is_last_two_swap, view_perm, view_shape
+from .views import is_identity, is_last_two_swap, view_data, view_perm, view_shape
 
 
 @dataclass(frozen=True)
@@ -236,7 +236,7 @@ class CudaDenseVariant(OpImplVariant):
         weight = input_tensor_for_role(node, 'rhs')
         bias = optional_tensor_for_role(node, 'bias')
         wi = to_quant_intent(weight.precision)
-        W = quantize_to_int(weight.data, wi.frac, wi.width, signed=wi.signed, rounding_mode=wi.rounding,
+        W = quantize_to_int(view_data(node, weight), wi.frac, wi.width, signed=wi.signed, rounding_mode=wi.rounding,
                             saturation_mode=wi.saturation)
         b = None
         if bias is not None:

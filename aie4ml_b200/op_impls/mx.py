@@ -22,7 +22,7 @@ from ..quant_utils import from_mx, to_mx
 from .base import CUDA_GENERATIONS, FamilyResolver, OpImplVariant, family_resolver, register_variant
 from .matmul import _transposed
 from .precision import ACTIVATION_CODE, resolve_exact_storage_dtype
-from .views import view_shape
+from .views import view_data, view_shape
 
 _ACTIVATION_FORMATS = ('bfloat16', 'float32')
 
@@ -48,8 +48,7 @@ def _precision(node: OpNode, weight_roles) -> Dict[str, AIEDataType]:
 
 def _pack_weights(node: OpNode, role: str):
     """-> (codes [N, pitch / 2], scale tiles, the float32 values [K, N] they stand for)"""
-    W = np.asarray(input_tensor_for_role(node, role).data, dtype=np.float64)
-    W = W.reshape(-1, W.shape[-2], W.shape[-1])[-1]
+    W = view_data(node, input_tensor_for_role(node, role))
     K, N = int(W.shape[0]), int(W.shape[1])
     codes, tiles = to_mx(np.ascontiguousarray(W.T))
     return codes, tiles, np.ascontiguousarray(from_mx(codes, tiles, N, K).T)
@@ -83,15 +82,15 @@ def _check_bias(node: OpNode, role: str, n_out: int) -> None:
         raise ValueError(f'{node.name}: {role} requires exactly {n_out} elements, got {int(np.asarray(bias.data).size)}.')
 
 
-def _check_extents(node: OpNode, weight, lhs_shape) -> None:
+def _check_extents(node: OpNode, weight_shape, lhs_shape) -> None:
     """What the kernels are told (n_in, n_out, the output's rows and columns) is what the tensors hold."""
     given = tuple(node.metadata.get(key) for key in ('n_in', 'n_out'))
-    if given != tuple(weight.shape):
-        raise ValueError(f'{node.name}: n_in and n_out {given} do not match the weight {tuple(weight.shape)}.')
+    if given != weight_shape:
+        raise ValueError(f'{node.name}: n_in and n_out {given} do not match the weight {weight_shape}.')
     out = tuple(int(d) for d in node.outputs[0].shape)
     rows = math.prod(lhs_shape[:-1])
-    if not out or out[-1] != weight.shape[1] or math.prod(out[:-1]) != rows:
-        raise ValueError(f'{node.name}: output {out} does not hold {rows} x {weight.shape[1]} results of the input {lhs_shape}.')
+    if not out or out[-1] != weight_shape[1] or math.prod(out[:-1]) != rows:
+        raise ValueError(f'{node.name}: output {out} does not hold {rows} x {weight_shape[1]} results of the input {lhs_shape}.')
 
 
 def _check_activation(node: OpNode, known) -> None:
@@ -106,12 +105,13 @@ class MxDenseFamilyResolver(FamilyResolver):
     def validate_structure(self, node, _device) -> None:
         lhs_shape = tuple(view_shape(node, input_tensor_for_role(node, 'lhs'), 'inputs'))
         weight = input_tensor_for_role(node, 'rhs')
+        shape = tuple(view_shape(node, weight, 'inputs'))
         if len(lhs_shape) < 2:
             raise ValueError(f'{node.name}: mx_dense requires a rank>=2 input, got {lhs_shape}.')
-        if not weight.is_parameter or len(weight.shape) != 2 or weight.shape[0] != lhs_shape[-1]:
-            raise ValueError(f'{node.name}: mx_dense needs a constant [K, N] weight that fits the input {lhs_shape}, got {weight.shape}.')
-        _check_extents(node, weight, lhs_shape)
-        _check_bias(node, 'bias', int(weight.shape[1]))
+        if not weight.is_parameter or len(shape) != 2 or shape[0] != lhs_shape[-1]:
+            raise ValueError(f'{node.name}: mx_dense needs a constant [K, N] weight that fits the input {lhs_shape}, got {shape}.')
+        _check_extents(node, shape, lhs_shape)
+        _check_bias(node, 'bias', shape[1])
         _check_activation(node, ('none', 'relu'))
 
 
@@ -154,11 +154,12 @@ class GatedDenseFamilyResolver(FamilyResolver):
             raise ValueError(f'{node.name}: gated_dense requires a rank>=2 input, got {lhs_shape}.')
         if not gate.is_parameter or not up.is_parameter:
             raise NotImplementedError(f'{node.name}: gated_dense needs constant weights.')
-        if len(gate.shape) != 2 or gate.shape != up.shape or gate.shape[0] != lhs_shape[-1]:
-            raise ValueError(f'{node.name}: gated_dense weights {gate.shape} and {up.shape} do not fit the input {lhs_shape}.')
-        _check_extents(node, gate, lhs_shape)
+        shape, up_shape = (tuple(view_shape(node, t, 'inputs')) for t in (gate, up))
+        if len(shape) != 2 or shape != up_shape or shape[0] != lhs_shape[-1]:
+            raise ValueError(f'{node.name}: gated_dense weights {shape} and {up_shape} do not fit the input {lhs_shape}.')
+        _check_extents(node, shape, lhs_shape)
         for role in ('gate_bias', 'up_bias'):
-            _check_bias(node, role, int(gate.shape[1]))
+            _check_bias(node, role, shape[1])
         _check_activation(node, ACTIVATION_CODE)
 
 

@@ -9,6 +9,8 @@ from __future__ import annotations
 
 from typing import Any, Dict, List, Optional
 
+import numpy as np
+
 from ..ir import TraitInstance
 
 MAX_RANK = 5
@@ -48,6 +50,13 @@ def view_shape(node, tensor, direction: str) -> List[int]:
     if sorted(perm) != list(range(len(logical))):
         raise ValueError(f'{node.name}: invalid io_view perm {perm} for rank {len(logical)}.')
     return [logical[i] for i in perm]
+
+
+def view_data(node, tensor) -> np.ndarray:
+    """A constant operand's values as the node sees them (a Transpose of the constant is folded like any other)."""
+    perm = view_perm(node, tensor, 'inputs')
+    data = np.asarray(tensor.data, dtype=np.float64)
+    return data if is_identity(perm) else np.ascontiguousarray(np.transpose(data, perm))
 
 
 def is_last_two_swap(perm: Optional[List[int]]) -> bool:
